@@ -251,6 +251,70 @@ int tops_f32_gated_mul(int64_t rows, int64_t cols, const float* a, int64_t lda, 
 int tops_transition_forward(int dtype, int64_t M, int64_t C, const void* x, const void* w12, const void* w3,
                             const float* b12, float eps, void* out, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * The sequence-local token block (no counterpart in the reference, whose attentions are dense
+ * and whose norms are folded into its projections): windowed attention with sinks, the norms
+ * around a block fused with its gate and residual scale, rotary positions. dtype: TOPS_F16,
+ * TOPS_BF16 or TOPS_F32. Strides count elements; pointers need only their type's alignment
+ * unless noted; zero sizes return TOPS_OK without a launch. */
+
+/* out = softmax(scale q k^T) v, where query i, at key position p = i + Nk - Nq, sees key j iff
+ *   j <= p + right  and  (j >= p - left  or  j < sinks)  and  (mask == NULL or mask[b*Nk + j]).
+ * q (B, Nq, Hq, D), k and v (B, Nk, Hkv, D), channels contiguous; strides[9] = {q: b, n, h;
+ * k: b, n, h; v: b, n, h}. Query head h reads key head h / (Hq / Hkv). Nq <= Nk, D <= 256.
+ * out [B][Nq][Hq][D]; lse [B][Hq][Nq] (natural log of the row sums; NULL: not wanted). A query
+ * that sees no key gets zeros and lse -inf. */
+int tops_window_attn_forward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
+                             const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask,
+                             int64_t left, int64_t right, int64_t sinks, float scale, void* out, float* lse,
+                             void* stream);
+/* Gradients dq [B][Nq][Hq][D], dk and dv [B][Nk][Hkv][D] from dout (dout_strides[3] = {b, n, h})
+ * and the forward's out and lse. workspace: 16-byte aligned, of the size that
+ * tops_window_attn_backward_workspace_bytes gives. Bitwise repeatable. */
+int tops_window_attn_backward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
+                              const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask,
+                              int64_t left, int64_t right, int64_t sinks, float scale, const void* dout,
+                              const int64_t* dout_strides, const void* out, const float* lse, void* workspace, void* dq,
+                              void* dk, void* dv, void* stream);
+int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv,
+                                              int64_t D, int64_t left, int64_t right, int64_t sinks, int64_t* bytes);
+/* One query for each of B sequences: q (B, Hq, D) at position min(lengths[b], N) - 1 of the caches
+ * k and v (B, N, Hkv, D); it sees the `window` newest keys and the first `sinks`. strides[8] =
+ * {q: b, h; k: b, n, h; v: b, n, h}; lengths int32 on the device (<= 0: zeros). out [B][Hq][D]. */
+int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, const void* q,
+                            const void* k, const void* v, const int64_t* strides, const int32_t* lengths,
+                            int64_t window, int64_t sinks, float scale, void* out, void* stream);
+
+/* u = post(y); r = u * sigmoid(gate); h = x + res_s * r; n = pre(h), over `rows` rows of C <= 8192
+ * channels (row strides xs, ys, gs); layer != 0: LayerNorm, else RMS norm. has_post, has_pre: the
+ * norms that there are. gate (NULL: none) has `groups` rows, each for rows/groups consecutive rows.
+ * Weights [C] of w_dtype (dtype or TOPS_F32), NULL for 1 (weights, res_s) or 0 (biases).
+ * h, n [rows][C]; stats [rows][4] fp32, 16-byte aligned (NULL: not wanted): mean, 1/std of y, of h. */
+int tops_gated_norm_forward(int dtype, int w_dtype, int64_t rows, int64_t groups, int64_t C, int layer, int has_post,
+                            int has_pre, float eps, const void* x, int64_t xs, const void* y, int64_t ys,
+                            const void* gate, int64_t gs, const void* post_w, const void* post_b, const void* res_s,
+                            const void* pre_w, const void* pre_b, void* h, void* n, float* stats, void* stream);
+/* Gradients from dh and dn (row strides dhs, dns; NULL: zero): dx, dy [rows][C], dgate [groups][C],
+ * and those of the weights [C] in w_dtype (NULL: not wanted). workspace: 16-byte aligned, of the
+ * size below. Bitwise repeatable. */
+int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, int64_t groups, int64_t C, int layer, int has_post,
+                             int has_pre, const void* dh, int64_t dhs, const void* dn, int64_t dns, const void* x,
+                             int64_t xs, const void* y, int64_t ys, const void* gate, int64_t gs, const float* stats,
+                             const void* post_w, const void* post_b, const void* res_s, const void* pre_w, void* dx,
+                             void* dy, void* dgate, void* dpost_w, void* dpost_b, void* dres_s, void* dpre_w,
+                             void* dpre_b, void* workspace, void* stream);
+int tops_gated_norm_backward_workspace_bytes(int64_t rows, int64_t groups, int64_t C, int64_t* bytes);
+
+/* Turns the channel pairs (f, D/2 + f), or (2f, 2f + 1) when interleaved, f < P <= D/2, of q
+ * (B, N, Hq, D) and k (B, N, Hk, D) by positions[axis[f]][b][n] * inv_freq[f] (negate: by the
+ * negated angle); other channels are copied. strides[6] = {q: b, n, h; k: b, n, h}; positions int32
+ * (wide: int64) with pos_strides[3] = {axis, b, n}; axis[f] outside 0..A-1 leaves the pair as it
+ * is. Outputs [B][N][H][D]; Hq or Hk may be 0. */
+int tops_rotary(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hk, int64_t D, int64_t P, int64_t A,
+                int interleaved, int negate, const void* q, const void* k, const int64_t* strides,
+                const void* positions, int wide, const int64_t* pos_strides, const float* inv_freq,
+                const int32_t* axis, void* q_out, void* k_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

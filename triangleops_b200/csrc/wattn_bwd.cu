@@ -1,0 +1,548 @@
+// wattn_bwd.cu — windowed attention with sinks, backward, on tcgen05 (what wattn.cu takes).
+//
+// With P = 2^(c S - lse2) from the saved log-sum-exp, delta_i = sum_d dO O and dP = dO v^T:
+//   dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,  dV = P^T dO.
+// Two kernels of one shape: 128 rows stay (two operand tiles A1, A2), tiles of 64 rows stream by
+// (B1, B2). Per streamed tile, T1 = A1 B1^T and T2 = A2 B2^T (fp32, TMEM); two softmax warpgroups,
+// taking tiles in turn, make P and dS from them and put them back to TMEM rounded to the IO dtype
+// (a product's operands have one type); then
+//   KV: rows are keys (A = k, v; B = q, dO):    dV += P B2,  dK += dS B1
+//   Q : rows are queries (A = q, dO; B = k, v): dQ += dS B1
+// accumulate in TMEM. T1 and T2 have two buffers, so the MMAs of one tile run under the softmax of
+// the other. S and dP are computed in both kernels (7 products for the 5 of one that adds dQ up in
+// memory by atomics): nothing is added in an order that changes, and dS is not stored.
+//
+// KV walks the query heads of its key head one after the other, so the sum over a shared head's
+// queries stays in TMEM. A block of sink keys is seen by every later query: its walk is cut into
+// `nch` parts of about the length of the other blocks', whose fp32 sums a last kernel adds in order.
+//
+// Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
+// before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
+// end, has lse2 = +inf, so that its P is 0.
+#include "sm100.cuh"
+#include "wattn.h"
+
+namespace tops {
+
+struct WattnBwdArgs {
+  int Nq, Nk, Hq, Hkv, group, D;
+  int left, right, sinks;
+  int tiles;             // Q: query tiles; KV: key tiles
+  int nsb, nch;          // KV: tiles with sinks, parts of their walk
+  int nqp;               // row length of lse2 and delta
+  const uint8_t* mask;
+  float c, scale;
+  const float *lse2, *delta;  // [B][Hq][nqp]
+  void *d1, *d2;              // KV: dv, dk; Q: dq
+  float* part;                // [B][Hkv][nsb][nch][2][128][DT]
+};
+
+template <int DT>
+struct WattnBwdCfg {
+  static constexpr int SUB = DT / 64;
+  static constexpr int RES = SUB * 128 * 128;  // bytes of a resident tile
+  static constexpr int STR = SUB * 64 * 128;   // bytes of a streamed tile
+  static constexpr int NST = 4;                // stages of streamed tiles
+  static constexpr int ACC = 256;              // TMEM: T1, T2 of buffer s at 128 s and 128 s + 64
+  static constexpr int THREADS = 320;
+};
+
+template <int DT>
+struct WattnBwdSmem {
+  using Cfg = WattnBwdCfg<DT>;
+  alignas(1024) uint8_t a1[Cfg::RES];
+  alignas(1024) uint8_t a2[Cfg::RES];
+  alignas(1024) uint8_t b1[Cfg::NST][Cfg::STR];
+  alignas(1024) uint8_t b2[Cfg::NST][Cfg::STR];
+  alignas(16) float st[Cfg::NST][2][64];  // KV: lse2 and delta of the streamed queries
+  uint64_t res_full, full[Cfg::NST], empty[Cfg::NST], t_full[2], ds_full[2], acc_done;
+  uint32_t tmem_base;
+  int abort;
+};
+
+// The walk of one block: which tiles stream by.
+template <bool KV>
+struct WattnWalk {
+  int b, row0, total;     // first resident row (key or query), streamed tiles
+  int head;               // KV: first query head of the group; Q: the query head
+  int hk, first, qlo, nqb, kb, chunk;
+  WattnBlocks<6> blk;     // Q: the key tiles
+  __device__ WattnWalk(const WattnBwdArgs& a) : blk(0, 1, 1, 0, 0, 0) {
+    if constexpr (KV) {
+      const int units = a.nsb * a.nch + a.tiles - a.nsb;
+      const int bh = blockIdx.x / units, u = blockIdx.x % units;
+      b = bh / a.Hkv;
+      hk = bh % a.Hkv;
+      head = hk * a.group;
+      const bool cut = u < a.nsb * a.nch;
+      kb = cut ? u / a.nch : u - a.nsb * a.nch + a.nsb;
+      chunk = cut ? u % a.nch : 0;
+      row0 = kb * 128;
+      const int off = a.Nk - a.Nq, last = min(row0 + 127, a.Nk - 1);
+      qlo = max(0, row0 - a.right - off) & ~7;
+      const int qhi = row0 < a.sinks ? a.Nq : min(a.Nq, last + a.left + 1 - off);
+      nqb = (max(0, qhi - qlo) + 63) >> 6;
+      const int64_t all = static_cast<int64_t>(nqb) * a.group;
+      const int parts = cut ? a.nch : 1;
+      first = static_cast<int>(all * chunk / parts);
+      total = static_cast<int>(all * (chunk + 1) / parts) - first;
+    } else {
+      const int tile = blockIdx.x % a.tiles;
+      head = blockIdx.x / a.tiles % a.Hq;
+      b = blockIdx.x / a.tiles / a.Hq;
+      hk = head / a.group;
+      row0 = tile * 128;
+      blk = WattnBlocks<6>(row0, a.Nq, a.Nk, a.left, a.right, a.sinks);
+      first = 0;
+      total = blk.n;
+      qlo = nqb = kb = chunk = 0;
+    }
+  }
+  // first row of streamed tile `it`, and its query head
+  __device__ int row(int it) const {
+    if constexpr (KV) return qlo + (first + it) % nqb * 64;
+    return blk.key(it);
+  }
+  __device__ int qhead(int it) const {
+    if constexpr (KV) return head + (first + it) / nqb;
+    return head;
+  }
+};
+
+template <typename T, int DT, bool KV>
+__global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
+    wattn_backward_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
+                          const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2,
+                          const WattnBwdArgs a) {
+  using Cfg = WattnBwdCfg<DT>;
+  using E = Elem<T>;
+  constexpr int NST = Cfg::NST, SUB = Cfg::SUB;
+  extern __shared__ uint8_t smem_raw[];
+  auto& sm = *reinterpret_cast<WattnBwdSmem<DT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort = &sm.abort;
+  const WattnWalk<KV> walk(a);
+
+  if (threadIdx.x == 0) {
+    mbar_init(&sm.res_full, 1);
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(&sm.full[s], 1);
+      mbar_init(&sm.empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sm.t_full[s], 1);
+      mbar_init(&sm.ds_full[s], 4);
+    }
+    mbar_init(&sm.acc_done, 1);
+    sm.abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(&sm.tmem_base, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = sm.tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0 && walk.total > 0) {
+      const int res_head = KV ? walk.hk : walk.head;
+      mbar_expect_tx(&sm.res_full, 2 * Cfg::RES);
+#pragma unroll
+      for (int s = 0; s < SUB; ++s) {
+        tma_load_4d(sm.a1 + s * 128 * 128, &map_a1, &sm.res_full, s * 64, res_head, walk.row0, walk.b);
+        tma_load_4d(sm.a2 + s * 128 * 128, &map_a2, &sm.res_full, s * 64, res_head, walk.row0, walk.b);
+      }
+      for (int it = 0; it < walk.total; ++it) {
+        const int r = it % NST;
+        if (!mbar_wait(&sm.empty[r], ((it / NST) & 1) ^ 1, abort, 521)) break;
+        const int row = walk.row(it), h = KV ? walk.qhead(it) : walk.hk;
+        mbar_expect_tx(&sm.full[r], 2 * Cfg::STR + (KV ? 512 : 0));
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+          tma_load_4d(sm.b1[r] + s * 64 * 128, &map_b1, &sm.full[r], s * 64, h, row, walk.b);
+          tma_load_4d(sm.b2[r] + s * 64 * 128, &map_b2, &sm.full[r], s * 64, h, row, walk.b);
+        }
+        if constexpr (KV) {
+          const int64_t at = (static_cast<int64_t>(walk.b) * a.Hq + h) * a.nqp + row;
+          bulk_load(sm.st[r][0], a.lse2 + at, 256, &sm.full[r]);
+          bulk_load(sm.st[r][1], a.delta + at, 256, &sm.full[r]);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && walk.total > 0) {
+      const uint32_t idesc_t = make_idesc_f16(128, 64, E::kFmt, false, false);
+      const uint32_t idesc_acc = make_idesc_f16(128, DT, E::kFmt, false, true);
+      const int ksteps = (a.D + 15) >> 4;
+      const uint32_t a1 = smem_u32(sm.a1), a2 = smem_u32(sm.a2);
+      auto issue_t = [&](int it) {
+        const int r = it % NST;
+        if (!mbar_wait(&sm.full[r], (it / NST) & 1, abort, 522)) return false;
+        tc_fence_after();
+        const uint32_t b1 = smem_u32(sm.b1[r]), b2 = smem_u32(sm.b2[r]);
+        const uint32_t t1 = tbase + (it & 1) * 128, t2 = t1 + 64;
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+          const uint32_t oa = (kk / 4) * 128 * 128 + (kk % 4) * 32, ob = (kk / 4) * 64 * 128 + (kk % 4) * 32;
+          if (kk < ksteps)
+            mma_ss(t1, make_smem_desc(a1 + oa, 16, 1024, kSw128), make_smem_desc(b1 + ob, 16, 1024, kSw128), idesc_t,
+                   kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < DT / 16; ++kk) {
+          const uint32_t oa = (kk / 4) * 128 * 128 + (kk % 4) * 32, ob = (kk / 4) * 64 * 128 + (kk % 4) * 32;
+          if (kk < ksteps)
+            mma_ss(t2, make_smem_desc(a2 + oa, 16, 1024, kSw128), make_smem_desc(b2 + ob, 16, 1024, kSw128), idesc_t,
+                   kk > 0);
+        }
+        mma_commit(&sm.t_full[it & 1]);
+        return true;
+      };
+      bool ok = mbar_wait(&sm.res_full, 0, abort, 523) && issue_t(0);
+      for (int it = 0; ok && it < walk.total; ++it) {
+        // T of the next tile: its buffer's P and dS were read by products issued before it
+        if (it + 1 < walk.total && !issue_t(it + 1)) break;
+        if (!mbar_wait(&sm.ds_full[it & 1], (it >> 1) & 1, abort, 524)) break;
+        tc_fence_after();
+        const int r = it % NST;
+        const uint32_t t1 = tbase + (it & 1) * 128, t2 = t1 + 64;
+        const uint32_t b1 = smem_u32(sm.b1[r]), b2 = smem_u32(sm.b2[r]);
+        if constexpr (KV) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ts(tbase + Cfg::ACC, t1 + kk * 8, make_smem_desc(b2 + kk * 2048, 8192, 1024, kSw128), idesc_acc,
+                   it > 0 || kk > 0);
+        }
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_ts(tbase + Cfg::ACC + (KV ? DT : 0), t2 + kk * 8, make_smem_desc(b1 + kk * 2048, 8192, 1024, kSw128),
+                 idesc_acc, it > 0 || kk > 0);
+        mma_commit(&sm.empty[r]);
+        if (it + 1 == walk.total) mma_commit(&sm.acc_done);
+      }
+    }
+  } else {
+    const int g = (warp - 2) >> 2;  // warpgroup: tiles g, g + 2, ...
+    const int wq = warp & 3;
+    const int row = wq * 32 + lane;
+    const uint32_t lane_addr = tbase + (static_cast<uint32_t>(wq * 32) << 16);
+    const int off = a.Nk - a.Nq;
+    // KV: this thread's key, and the positions [plo, phi) that see it; Q: its query's position and
+    // the keys [lo, hi) of its window
+    const int at = walk.row0 + row;
+    int lo, hi, upto = 0;
+    bool keep = true;
+    float lse2 = 0.f, delta = 0.f;
+    if constexpr (KV) {
+      lo = at - a.right;
+      hi = at < a.sinks ? a.Nk : at + a.left + 1;
+      if (a.mask && at < a.Nk) keep = a.mask[static_cast<int64_t>(walk.b) * a.Nk + at] != 0;
+    } else {
+      const int p = at + off;
+      lo = p - a.left;
+      hi = min(p + a.right + 1, a.Nk);
+      upto = a.sinks;
+      // nqp reaches past the last tile's rows: those hold +inf and 0
+      const int64_t q = (static_cast<int64_t>(walk.b) * a.Hq + walk.head) * a.nqp + at;
+      lse2 = a.lse2[q];
+      delta = a.delta[q];
+    }
+    const unsigned long long c2 = f2_pack(a.c, a.c);
+    bool ok = true;
+    for (int it = g; it < walk.total; it += 2) {
+      const int r = it % NST, r0 = walk.row(it);
+      uint32_t kept[2] = {0xffffffffu, 0xffffffffu};
+      bool whole = keep;
+      if (!KV && a.mask) {
+        const uint8_t* mk = a.mask + static_cast<int64_t>(walk.b) * a.Nk;
+        uint8_t byte[2];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const int k = r0 + w * 32 + lane;
+          byte[w] = k < a.Nk ? mk[k] : 0;
+        }
+        kept[0] = __ballot_sync(0xffffffffu, byte[0] != 0);
+        kept[1] = __ballot_sync(0xffffffffu, byte[1] != 0);
+        whole = (kept[0] & kept[1]) == 0xffffffffu;
+      }
+      if (KV && !mbar_wait(&sm.full[r], (it / NST) & 1, abort, 525)) { ok = false; break; }
+      if (!mbar_wait(&sm.t_full[g], (it >> 1) & 1, abort, 526)) { ok = false; break; }
+      tc_fence_after();
+      uint32_t x[64], y[64];
+      const uint32_t t1 = lane_addr + g * 128, t2 = t1 + 64;
+      tmem_ld64_async(t1, x);
+      tmem_ld64_async(t2, y);
+      tmem_wait_ld64(x);
+      tmem_wait_ld64(y);
+      bool inside;
+      if constexpr (KV) {
+        const int p0 = r0 + off;
+        inside = p0 >= walk.row0 + 127 - a.right && p0 + 63 <= walk.row0 + a.left;
+      } else {
+        const int p0 = walk.row0 + off;
+        inside = r0 + 64 <= min(p0 + a.right + 1, a.Nk) && !walk.blk.sink(it) &&
+                 (r0 >= p0 + walk.blk.rows - 1 - a.left || r0 + 64 <= a.sinks);
+      }
+      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      const bool edge = __any_sync(0xffffffffu, !inside || !whole);
+      if (edge) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if constexpr (KV) {
+            const int b0 = r0 + off + w * 32;
+            see[w] = keep ? bits_below(hi - b0) & ~bits_below(lo - b0) : 0u;
+          } else {
+            const int b0 = r0 + w * 32;
+            const bool snk = walk.blk.sink(it);
+            const int f = snk ? walk.blk.nse : lo, u = snk ? walk.blk.nse : upto;
+            see[w] = bits_below(hi - b0) & (~bits_below(f - b0) | bits_below(u - b0)) & kept[w];
+            if (snk) see[w] &= bits_below(walk.blk.nse - b0);
+          }
+        }
+      }
+      const float* s_lse = sm.st[r][0];
+      const float* s_del = sm.st[r][1];
+#pragma unroll
+      for (int c0 = 0; c0 < 64; c0 += 32) {
+        uint32_t pk[16], dk[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = c0 + 2 * i;
+          unsigned long long nl, nd;
+          if constexpr (KV) {
+            nl = f2_pack(-s_lse[e], -s_lse[e + 1]);
+            nd = f2_pack(-s_del[e], -s_del[e + 1]);
+          } else {
+            nl = f2_pack(-lse2, -lse2);
+            nd = f2_pack(-delta, -delta);
+          }
+          float p0, p1, d0, d1;
+          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, nl), p0, p1);
+          p0 = ex2_approx(p0);
+          p1 = ex2_approx(p1);
+          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), nd), f2_pack(p0, p1)), d0,
+                    d1);
+          if (edge) {
+            const uint32_t w = see[c0 / 32] >> (2 * i);
+            if (!(w & 1)) p0 = d0 = 0.f;
+            if (!(w & 2)) p1 = d1 = 0.f;
+          }
+          if constexpr (KV) pk[i] = E::pack2(p0, p1);
+          dk[i] = E::pack2(d0, d1);
+        }
+        if constexpr (KV) tmem_st16(t1 + c0 / 2, pk);
+        tmem_st16(t2 + c0 / 2, dk);
+      }
+      if (!KV && a.mask && !whole) {
+        // T1 of this tile is done: its masked keys' rows may be zeroed for dS k
+        const uint32_t word = row < 32 ? kept[0] : kept[1];
+        if (row < 64 && !(word >> lane & 1)) {
+#pragma unroll
+          for (int s = 0; s < SUB; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              reinterpret_cast<uint4*>(sm.b1[r] + s * 64 * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.ds_full[g]);
+    }
+    // ---------------- epilogue ----------------
+    // KV: warpgroup 0 writes dV, 1 dK; Q: each half of dQ's channels
+    if (walk.total > 0 && (!ok || !mbar_wait(&sm.acc_done, 0, abort, 527))) ok = false;
+    if (ok) {
+      tc_fence_after();
+      const float f = KV && g == 0 ? 1.f : a.scale;
+      const bool zero = walk.total == 0;
+      constexpr int COLS = KV ? DT : DT / 2;
+      const int col0 = KV ? 0 : g * COLS;
+      const uint32_t acc = lane_addr + Cfg::ACC + (KV ? g * DT : col0);
+      float* part = nullptr;
+      T* dst;
+      if constexpr (KV) {
+        if (a.nch > 1 && walk.kb < a.nsb)
+          part = a.part +
+                 ((((static_cast<int64_t>(walk.b) * a.Hkv + walk.hk) * a.nsb + walk.kb) * a.nch + walk.chunk) * 2 + g) *
+                     128 * DT +
+                 row * DT;
+        dst = static_cast<T*>(g == 0 ? a.d1 : a.d2) + ((static_cast<int64_t>(walk.b) * a.Nk + at) * a.Hkv + walk.hk) * a.D;
+      } else {
+        dst = static_cast<T*>(a.d1) + ((static_cast<int64_t>(walk.b) * a.Nq + at) * a.Hq + walk.head) * a.D + col0;
+      }
+      const bool live = at < (KV ? a.Nk : a.Nq);
+#pragma unroll
+      for (int c0 = 0; c0 < COLS; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32(acc + c0, o);
+        if (zero)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        if (KV && part != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *reinterpret_cast<uint4*>(part + c0 + 4 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if (live) {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            uint32_t pk[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              pk[e] = E::pack2(__uint_as_float(o[8 * v + 2 * e]) * f, __uint_as_float(o[8 * v + 2 * e + 1]) * f);
+            if (col0 + c0 + 8 * v < a.D)
+              *reinterpret_cast<uint4*>(dst + c0 + 8 * v) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tbase, 512);
+}
+
+// delta = sum_d dO O and lse2 = lse log2(e) per query, in rows of nqp: queries past Nq, and those
+// that see nothing, get lse2 = +inf and delta = 0. Eight threads a query, 16-byte loads.
+template <typename T>
+__global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* __restrict__ dout, int64_t s0,
+                                                          int64_t s1, int64_t s2, const T* __restrict__ out,
+                                                          const float* __restrict__ lse, int nqp,
+                                                          float* __restrict__ lse2, float* __restrict__ delta) {
+  using E = Elem<T>;
+  const int i = static_cast<int>((blockIdx.x * 256u + threadIdx.x) >> 3), part = threadIdx.x & 7;
+  const int h = blockIdx.y, b = blockIdx.z;
+  float x = 0.f;
+  if (i < a.Nq) {
+    const T* d = dout + b * s0 + i * s1 + h * s2;
+    const T* o = out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D;
+    for (int c = part * 8; c < a.D; c += 64) {
+      const uint4 u = *reinterpret_cast<const uint4*>(d + c), w = *reinterpret_cast<const uint4*>(o + c);
+      x = fmaf(E::lo(u.x), E::lo(w.x), fmaf(E::hi(u.x), E::hi(w.x), x));
+      x = fmaf(E::lo(u.y), E::lo(w.y), fmaf(E::hi(u.y), E::hi(w.y), x));
+      x = fmaf(E::lo(u.z), E::lo(w.z), fmaf(E::hi(u.z), E::hi(w.z), x));
+      x = fmaf(E::lo(u.w), E::lo(w.w), fmaf(E::hi(u.w), E::hi(w.w), x));
+    }
+  }
+#pragma unroll
+  for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  if (part == 0 && i < nqp) {
+    const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
+    const float v = i < a.Nq ? lse[bh * a.Nq + i] : -INFINITY;
+    lse2[bh * nqp + i] = v == -INFINITY ? INFINITY : v * kLog2e;
+    delta[bh * nqp + i] = v == -INFINITY ? 0.f : x;
+  }
+}
+
+// Adds the parts of the sink tiles' walks, in order. One block a (b, key head, tile, output, 8 rows).
+template <typename T, int DT>
+__global__ void __launch_bounds__(256) wattn_parts_kernel(WattnBwdArgs a) {
+  using E = Elem<T>;
+  constexpr int PER = DT / 8;  // threads a row, 8 channels each
+  constexpr int ROWS = 256 / PER;
+  const int row = blockIdx.x * ROWS + threadIdx.x / PER, col = threadIdx.x % PER * 8;
+  const int which = blockIdx.y & 1, kb = blockIdx.y >> 1;
+  const int64_t bh = blockIdx.z;
+  const int key = kb * 128 + row;
+  if (row >= 128 || key >= a.Nk || col >= a.D) return;
+  const float* p = a.part + ((bh * a.nsb + kb) * a.nch * 2 + which) * 128 * DT + row * DT + col;
+  float v[8] = {};
+  for (int n = 0; n < a.nch; ++n, p += 2 * 128 * DT) {
+    const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
+    v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
+    v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
+  }
+  const float f = which == 0 ? 1.f : a.scale;
+  const int64_t b = bh / a.Hkv, hk = bh % a.Hkv;
+  T* dst = static_cast<T*>(which == 0 ? a.d1 : a.d2) + ((b * a.Nk + key) * a.Hkv + hk) * a.D + col;
+  *reinterpret_cast<uint4*>(dst) = make_uint4(E::pack2(v[0] * f, v[1] * f), E::pack2(v[2] * f, v[3] * f),
+                                              E::pack2(v[4] * f, v[5] * f), E::pack2(v[6] * f, v[7] * f));
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+struct WattnBwdPlan {
+  int nqp, nsb, nch;
+  int64_t stats, part;  // elements of each of lse2 and delta; of the sink tiles' parts
+};
+
+inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
+  WattnBwdPlan p;
+  // a streamed tile starts at a multiple of 8 below Nq and reads 64, a resident one 128
+  p.nqp = static_cast<int>((Nq + 127) / 128 * 128 + 64);
+  p.stats = static_cast<int64_t>(a.B) * a.Hq * p.nqp;
+  const int group = a.Hq / a.Hkv;
+  p.nsb = (a.sinks + 127) / 128;
+  const int64_t all = group * ((Nq + 63) / 64);
+  int64_t own = static_cast<int64_t>(a.left) + a.right + 128;
+  own = group * ((own + 63) / 64);
+  if (own < 8) own = 8;
+  int64_t nch = p.nsb > 0 ? (all + own - 1) / own : 1;
+  p.nch = static_cast<int>(nch < 1 ? 1 : nch > 64 ? 64 : nch);
+  if (p.nch == 1) p.nsb = 0;
+  const int64_t DT = a.D <= 64 ? 64 : 128;
+  p.part = p.nsb > 0 ? static_cast<int64_t>(a.B) * a.Hkv * p.nsb * p.nch * 2 * 128 * DT : 0;
+  return p;
+}
+
+template <typename T, int DT>
+int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
+                          const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
+  const WattnBwdPlan p = wattn_bwd_plan(a, a.Nq);
+  float *lse2 = ws, *delta = ws + p.stats;
+  if (a.Hq > 65535 || a.B > 65535) return TOPS_ERR_SHAPE;
+  wattn_stats_kernel<T><<<dim3((p.nqp + 31) / 32, a.Hq, a.B), 256, 0, st>>>(
+      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
+  CUtensorMap q128, k128, v128, d128, q64, k64, v64, d64;
+  if (!wattn_map(&q128, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 128) ||
+      !wattn_map(&d128, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 128) ||
+      !wattn_map(&k128, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 128) ||
+      !wattn_map(&v128, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 128) ||
+      !wattn_map(&q64, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 64) ||
+      !wattn_map(&d64, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 64) ||
+      !wattn_map(&k64, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 64) ||
+      !wattn_map(&v64, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64))
+    return TOPS_ERR_TMAP;
+  WattnBwdArgs f;
+  f.Nq = a.Nq, f.Nk = a.Nk, f.Hq = a.Hq, f.Hkv = a.Hkv, f.group = a.Hq / a.Hkv, f.D = a.D;
+  f.left = a.left, f.right = a.right, f.sinks = a.sinks;
+  f.nsb = p.nsb, f.nch = p.nch, f.nqp = p.nqp, f.mask = a.mask;
+  f.c = a.scale * kLog2e, f.scale = a.scale, f.lse2 = lse2, f.delta = delta;
+  f.part = ws + 2 * p.stats;
+  const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
+  {
+    f.tiles = (a.Nk + 127) / 128;
+    f.d1 = dv, f.d2 = dk;
+    const int64_t grid = (static_cast<int64_t>(f.nsb) * f.nch + f.tiles - f.nsb) * a.Hkv * a.B;
+    if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+    auto kern = wattn_backward_kernel<T, DT, true>;
+    set_smem(kern, smem);
+    kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(k128, v128, q64, d64, f);
+    if (const int rc = launch_status()) return rc;
+    if (f.nsb > 0) {
+      constexpr int ROWS = 256 / (DT / 8);
+      if (static_cast<int64_t>(a.B) * a.Hkv > 65535 || f.nsb > 32767) return TOPS_ERR_SHAPE;
+      wattn_parts_kernel<T, DT><<<dim3(128 / ROWS, 2 * f.nsb, a.B * a.Hkv), 256, 0, st>>>(f);
+      if (const int rc = launch_status()) return rc;
+    }
+  }
+  f.tiles = (a.Nq + 127) / 128;
+  f.d1 = dq, f.d2 = nullptr;
+  const int64_t grid = static_cast<int64_t>(f.tiles) * a.Hq * a.B;
+  if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  auto kern = wattn_backward_kernel<T, DT, false>;
+  set_smem(kern, smem);
+  kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(q128, d128, k64, v64, f);
+  return launch_status();
+}
+
+template <typename T>
+int run_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
+                       const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
+  return a.D <= 64 ? launch_wattn_backward<T, 64>(dtype, a, dout, ds, out, lse, ws, dq, dk, dv, st)
+                   : launch_wattn_backward<T, 128>(dtype, a, dout, ds, out, lse, ws, dq, dk, dv, st);
+}
+
+}  // namespace tops
