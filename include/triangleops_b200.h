@@ -280,10 +280,13 @@ int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, int64_t Nq, 
                                               int64_t D, int64_t left, int64_t right, int64_t sinks, int64_t* bytes);
 /* One query for each of B sequences: q (B, Hq, D) at position min(lengths[b], N) - 1 of the caches
  * k and v (B, N, Hkv, D); it sees the `window` newest keys and the first `sinks`. strides[8] =
- * {q: b, h; k: b, n, h; v: b, n, h}; lengths int32 on the device (<= 0: zeros). out [B][Hq][D]. */
+ * {q: b, h; k: b, n, h; v: b, n, h}; lengths int32 on the device (<= 0: zeros). out [B][Hq][D].
+ * workspace: 16-byte aligned, of the size below (often 0: NULL will do). */
 int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, const void* q,
                             const void* k, const void* v, const int64_t* strides, const int32_t* lengths,
-                            int64_t window, int64_t sinks, float scale, void* out, void* stream);
+                            int64_t window, int64_t sinks, float scale, void* workspace, void* out, void* stream);
+int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                            int64_t sinks, int64_t* bytes);
 
 /* u = post(y); r = u * sigmoid(gate); h = x + res_s * r; n = pre(h), over `rows` rows of C <= 8192
  * channels (row strides xs, ys, gs); layer != 0: LayerNorm, else RMS norm. has_post, has_pre: the

@@ -109,10 +109,18 @@ extern "C" int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, i
   return TOPS_OK;
 }
 
+extern "C" int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
+                                                       int64_t window, int64_t sinks, int64_t* bytes) {
+  if (bytes == nullptr || window < 1 || sinks < 0) return TOPS_ERR_ARG;
+  if (B < 0 || N < 1 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return TOPS_ERR_SHAPE;
+  *bytes = wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
+  return TOPS_OK;
+}
+
 extern "C" int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
                                        const void* q, const void* k, const void* v, const int64_t* strides,
-                                       const int32_t* lengths, int64_t window, int64_t sinks, float scale, void* out,
-                                       void* stream) {
+                                       const int32_t* lengths, int64_t window, int64_t sinks, float scale,
+                                       void* workspace, void* out, void* stream) {
   if (dtype != TOPS_BF16 && dtype != TOPS_F16 && dtype != TOPS_F32) return TOPS_ERR_DTYPE;
   if (window < 1) return TOPS_ERR_ARG;
   if (N < 1) return TOPS_ERR_SHAPE;
@@ -125,5 +133,11 @@ extern "C" int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t 
   if (lengths == nullptr || out == nullptr) return TOPS_ERR_ARG;
   a.lengths = lengths;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype != TOPS_F32 && D % 8 == 0 && D <= 128 && wattn_decode_rows(q, a.qs[0], a.qs[2], 0) &&
+      wattn_decode_rows(k, a.ks[0], a.ks[1], a.ks[2]) && wattn_decode_rows(v, a.vs[0], a.vs[1], a.vs[2])) {
+    float* part = static_cast<float*>(workspace);
+    return dtype == TOPS_BF16 ? run_wattn_decode<__nv_bfloat16>(a, window, out, part, st)
+                              : run_wattn_decode<__half>(a, window, out, part, st);
+  }
   return by_io_type(dtype, [&](auto t) { return run_wattn_generic<decltype(t)>(a, out, nullptr, st); });
 }

@@ -46,18 +46,8 @@ struct GnormArgs {
   int tpr;                 // threads to a row
 };
 
-constexpr int kGnVals = 8;  // channels per thread
-
-template <typename T, int VEC>
-struct Pack;  // VEC values of T as they lie in memory
-template <typename T>
-struct Pack<T, 8> {
-  using type = uint4;
-};
-template <>
-struct Pack<float, 4> {
-  using type = float4;
-};
+constexpr int kGnVals = 8;  // channels per thread, held as 4 pairs (packed fp32 arithmetic)
+using f2 = unsigned long long;
 
 // channel of value i (0..7) of the thread at `t` of a row of tpr threads
 template <int VEC>
@@ -65,29 +55,52 @@ __device__ __forceinline__ int gn_channel(int t, int tpr, int i) {
   return (t + (i / VEC) * tpr) * VEC + i % VEC;
 }
 
+// A thread's 8 channels as they lie in memory: 16-byte pieces of VEC values, or (VEC 1) one by
+// one. Channels past C are zero.
 template <typename T, int VEC>
-__device__ __forceinline__ void gn_load(const T* p, int t, int tpr, int C, float* f) {
+struct GnRaw {
+  uint4 w[8 / VEC];
+  __device__ __forceinline__ void load(const T* p, int t, int tpr, int C) {
 #pragma unroll
-  for (int k = 0; k < kGnVals / VEC; ++k) {
-    const int c = (t + k * tpr) * VEC;
-    if constexpr (VEC == 1) {
-      f[k] = c < C ? static_cast<float>(p[c]) : 0.f;
-    } else {
-      typename Pack<T, VEC>::type w{};
-      if (c < C) w = *reinterpret_cast<const typename Pack<T, VEC>::type*>(p + c);
-      if constexpr (sizeof(T) == 4) {
-        f[4 * k] = w.x, f[4 * k + 1] = w.y, f[4 * k + 2] = w.z, f[4 * k + 3] = w.w;
-      } else {
-        using E = Elem<T>;
-        f[0] = E::lo(w.x), f[1] = E::hi(w.x), f[2] = E::lo(w.y), f[3] = E::hi(w.y);
-        f[4] = E::lo(w.z), f[5] = E::hi(w.z), f[6] = E::lo(w.w), f[7] = E::hi(w.w);
-      }
+    for (int k = 0; k < 8 / VEC; ++k) {
+      const int c = (t + k * tpr) * VEC;
+      w[k] = c < C ? *reinterpret_cast<const uint4*>(p + c) : make_uint4(0, 0, 0, 0);
     }
   }
-}
+  __device__ __forceinline__ void get(f2* f) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        f[2 * k] = f2_pack(__uint_as_float(w[k].x), __uint_as_float(w[k].y));
+        f[2 * k + 1] = f2_pack(__uint_as_float(w[k].z), __uint_as_float(w[k].w));
+      }
+    } else {
+      using E = Elem<T>;
+      f[0] = f2_pack(E::lo(w[0].x), E::hi(w[0].x));
+      f[1] = f2_pack(E::lo(w[0].y), E::hi(w[0].y));
+      f[2] = f2_pack(E::lo(w[0].z), E::hi(w[0].z));
+      f[3] = f2_pack(E::lo(w[0].w), E::hi(w[0].w));
+    }
+  }
+};
+template <typename T>
+struct GnRaw<T, 1> {
+  T v[8];
+  __device__ __forceinline__ void load(const T* p, int t, int tpr, int C) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = t + i * tpr < C ? p[t + i * tpr] : T(0.f);
+  }
+  __device__ __forceinline__ void get(f2* f) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = f2_pack(static_cast<float>(v[2 * i]), static_cast<float>(v[2 * i + 1]));
+  }
+};
 
 template <typename T, int VEC>
-__device__ __forceinline__ void gn_store(T* p, int t, int tpr, int C, const float* f) {
+__device__ __forceinline__ void gn_store(T* p, int t, int tpr, int C, const f2* v) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_unpack(v[i], f[2 * i], f[2 * i + 1]);
 #pragma unroll
   for (int k = 0; k < kGnVals / VEC; ++k) {
     const int c = (t + k * tpr) * VEC;
@@ -104,44 +117,51 @@ __device__ __forceinline__ void gn_store(T* p, int t, int tpr, int C, const floa
   }
 }
 
-// a weight row of either dtype (read once a block)
+// A weight row of either dtype, read once a block. Channels past C get 0, whatever the default:
+// then nothing of theirs enters a sum.
 template <typename T, int VEC>
-__device__ __forceinline__ void gn_weight(const void* w, int io, int t, int tpr, int C, float none, float* f) {
+__device__ __forceinline__ void gn_weight(const void* w, int io, int t, int tpr, int C, float none, f2* f) {
+  float v[8];
 #pragma unroll
   for (int i = 0; i < kGnVals; ++i) {
     const int c = gn_channel<VEC>(t, tpr, i);
-    f[i] = none;
+    v[i] = c < C ? none : 0.f;
     if (w != nullptr && c < C)
-      f[i] = io ? static_cast<float>(static_cast<const T*>(w)[c]) : static_cast<const float*>(w)[c];
+      v[i] = io ? static_cast<float>(static_cast<const T*>(w)[c]) : static_cast<const float*>(w)[c];
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = f2_pack(v[2 * i], v[2 * i + 1]);
 }
 
-// Sums of two values over the threads of a row. MULTI: the row takes the whole block; `red` is
-// then two buffers of 2 x 32 floats used in turn, so that one barrier a sum is enough.
-template <bool MULTI>
-__device__ __forceinline__ float2 row_sum(float a, float b, int tpr, float* red, int& turn) {
+__device__ __forceinline__ f2 f2_both(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ float f2_sum(f2 v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
+
+// Sums of N values over the threads of a row. MULTI: the row takes the whole block; `red` is then
+// two buffers of N x 32 floats used in turn, so that one barrier a sum is enough.
+template <bool MULTI, int N>
+__device__ __forceinline__ void row_sum(float* v, int tpr, float* red, int& turn) {
   const int width = MULTI ? 32 : tpr;
-  for (int o = width >> 1; o; o >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, o);
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-  }
+  for (int o = width >> 1; o; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   if constexpr (MULTI) {
     float* r = red + (turn ^= 1) * 64;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    if (lane == 0) {
-      r[warp] = a;
-      r[32 + warp] = b;
-    }
-    __syncthreads();
-    a = lane < nw ? r[lane] : 0.f;
-    b = lane < nw ? r[32 + lane] : 0.f;
+    if (lane == 0)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      a += __shfl_xor_sync(0xffffffffu, a, o);
-      b += __shfl_xor_sync(0xffffffffu, b, o);
+      for (int i = 0; i < N; ++i) r[32 * i + warp] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = lane < nw ? r[32 * i + lane] : 0.f;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     }
   }
-  return make_float2(a, b);
 }
 
 // 16-bit IO: two ulps of the hardware's exponential and quotient are far below its rounding
@@ -152,202 +172,259 @@ __device__ __forceinline__ float gn_sigmoid(float x) {
   else
     return __fdividef(1.f, 1.f + __expf(-x));  // 0 once the divisor passes 2^126
 }
-// 1/sqrt, to the last bit but one where the IO shows it
 template <typename T>
-__device__ __forceinline__ float gn_rsqrt(float x) {
-  return sizeof(T) == 4 ? 1.f / sqrtf(x) : rsqrtf(x);
+__device__ __forceinline__ f2 gn_sigmoid2(f2 x) {
+  float a, b;
+  f2_unpack(x, a, b);
+  return f2_pack(gn_sigmoid<T>(a), gn_sigmoid<T>(b));
 }
 
 // mean and 1/std of a row's values (rms: mean 0)
 template <typename T, int VEC, bool MULTI>
-__device__ __forceinline__ float2 gn_stats(const float* f, int t, const GnormArgs& a, float* red, int& turn) {
+__device__ __forceinline__ float2 gn_stats(const f2* f, int t, const GnormArgs& a, float* red, int& turn) {
   const float inv = 1.f / a.C;
-  float mean = 0.f, s = 0.f;
+  float mean = 0.f, s;
   if (a.layer) {
-#pragma unroll
-    for (int i = 0; i < kGnVals; ++i) s += f[i];  // channels past C hold 0
-    mean = row_sum<MULTI>(s, 0.f, a.tpr, red, turn).x * inv;
+    s = f2_sum(f2_add(f2_add(f[0], f[1]), f2_add(f[2], f[3])));  // channels past C hold 0
+    row_sum<MULTI, 1>(&s, a.tpr, red, turn);
+    mean = s * inv;
   }
-  s = 0.f;
+  f2 acc = 0;
 #pragma unroll
-  for (int i = 0; i < kGnVals; ++i) {
-    const float d = gn_channel<VEC>(t, a.tpr, i) < a.C ? f[i] - mean : 0.f;
-    s = fmaf(d, d, s);
+  for (int i = 0; i < 4; ++i) {
+    const float m0 = gn_channel<VEC>(t, a.tpr, 2 * i) < a.C ? mean : 0.f;
+    const float m1 = VEC > 1 ? m0 : gn_channel<VEC>(t, a.tpr, 2 * i + 1) < a.C ? mean : 0.f;
+    const f2 d = f2_add(f[i], f2_pack(-m0, -m1));
+    acc = f2_fma(d, d, acc);
   }
-  return make_float2(mean, gn_rsqrt<T>(row_sum<MULTI>(s, 0.f, a.tpr, red, turn).x * inv + a.eps));
+  s = f2_sum(acc);
+  row_sum<MULTI, 1>(&s, a.tpr, red, turn);
+  s = fmaf(s, inv, a.eps);
+  return make_float2(mean, sizeof(T) == 4 ? 1.f / sqrtf(s) : rsqrtf(s));
 }
 
 // Threads of a block, at most THREADS: rows side by side, a.tpr threads each, or (more than 128)
-// one row. Block b takes rows
-// b * slots + slot, then on by the grid.
+// one row. Block b takes rows b * slots + slot, then on by the grid; the next row's values are on
+// their way while the present one's are worked on.
 template <typename T, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS) gnorm_forward_kernel(GnormArgs a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 && VEC > 1 ? 5 : 1) gnorm_forward_kernel(GnormArgs a) {
   constexpr bool MULTI = THREADS > 128;
   __shared__ float red[MULTI ? 128 : 1];
   int turn = 0;
   const int tpr = a.tpr, t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = blockDim.x / tpr, C = a.C;
-  float pw[kGnVals], pb[kGnVals], sc[kGnVals], nw[kGnVals], nb[kGnVals];
+  f2 pw[4], pb[4], sc[4], nw[4], nb[4];
   gn_weight<T, VEC>(a.post_w, a.w_io, t, tpr, C, 1.f, pw);
   gn_weight<T, VEC>(a.post_b, a.w_io, t, tpr, C, 0.f, pb);
   gn_weight<T, VEC>(a.res_s, a.w_io, t, tpr, C, 1.f, sc);
   gn_weight<T, VEC>(a.pre_w, a.w_io, t, tpr, C, 1.f, nw);
   gn_weight<T, VEC>(a.pre_b, a.w_io, t, tpr, C, 0.f, nb);
   const int64_t step = static_cast<int64_t>(gridDim.x) * slots;
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * slots; r0 < a.rows; r0 += step) {
-    const bool live = r0 + slot < a.rows;  // the others keep up with the warp's shuffles
-    const int64_t r = live ? r0 + slot : a.rows - 1;
-    float x[kGnVals], y[kGnVals], g[kGnVals];
-    gn_load<T, VEC>(static_cast<const T*>(a.x) + r * a.xs, t, tpr, C, x);
-    gn_load<T, VEC>(static_cast<const T*>(a.y) + r * a.ys, t, tpr, C, y);
-    if (a.gate) gn_load<T, VEC>(static_cast<const T*>(a.gate) + (a.shared ? r / a.group_rows : r) * a.gs, t, tpr, C, g);
+  GnRaw<T, VEC> rx, ry, rg;
+  auto load = [&](int64_t r) {
+    r = r < a.rows ? r : a.rows - 1;  // a thread without a row keeps up with its warp's shuffles
+    rx.load(static_cast<const T*>(a.x) + r * a.xs, t, tpr, C);
+    ry.load(static_cast<const T*>(a.y) + r * a.ys, t, tpr, C);
+    if (a.gate) rg.load(static_cast<const T*>(a.gate) + (a.shared ? r / a.group_rows : r) * a.gs, t, tpr, C);
+  };
+  int64_t r0 = static_cast<int64_t>(blockIdx.x) * slots;
+  if (r0 < a.rows) load(r0 + slot);
+  for (; r0 < a.rows; r0 += step) {
+    const int64_t r = r0 + slot;
+    const bool live = r < a.rows;
+    f2 x[4], y[4], g[4];
+    rx.get(x);
+    ry.get(y);
+    if (a.gate) rg.get(g);
+    if (r0 + step < a.rows) load(r + step);
     float2 sy = make_float2(0.f, 1.f), sh = sy;
-    if (a.has_post) sy = gn_stats<T, VEC, MULTI>(y, t, a, red, turn);
+    if (a.has_post) {
+      sy = gn_stats<T, VEC, MULTI>(y, t, a, red, turn);
+      const f2 m = f2_both(-sy.x), q = f2_both(sy.y);
 #pragma unroll
-    for (int i = 0; i < kGnVals; ++i) {
-      float u = a.has_post ? fmaf((y[i] - sy.x) * sy.y, pw[i], pb[i]) : y[i];
-      if (a.gate) u *= gn_sigmoid<T>(g[i]);
-      x[i] = gn_channel<VEC>(t, tpr, i) < C ? fmaf(sc[i], u, x[i]) : 0.f;  // h
+      for (int i = 0; i < 4; ++i) y[i] = f2_fma(f2_mul(f2_add(y[i], m), q), pw[i], pb[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (a.gate) y[i] = f2_mul(y[i], gn_sigmoid2<T>(g[i]));
+      x[i] = f2_fma(sc[i], y[i], x[i]);  // h
     }
     if (live) gn_store<T, VEC>(static_cast<T*>(a.h) + r * C, t, tpr, C, x);
     if (a.has_pre) {
       sh = gn_stats<T, VEC, MULTI>(x, t, a, red, turn);
+      const f2 m = f2_both(-sh.x), q = f2_both(sh.y);
 #pragma unroll
-      for (int i = 0; i < kGnVals; ++i) x[i] = fmaf((x[i] - sh.x) * sh.y, nw[i], nb[i]);
+      for (int i = 0; i < 4; ++i) x[i] = f2_fma(f2_mul(f2_add(x[i], m), q), nw[i], nb[i]);
       if (live) gn_store<T, VEC>(static_cast<T*>(a.n) + r * C, t, tpr, C, x);
     }
     if (live && a.stats && t == 0) reinterpret_cast<float4*>(a.stats)[r] = make_float4(sy.x, sy.y, sh.x, sh.y);
   }
 }
 
-// Adds each thread's 8 sums over the block's row slots; slot 0 is left with the total.
-template <int VEC>
-__device__ __forceinline__ void slot_sum(float* f, float* buf, int t, int slot, int slots, int tpr) {
+// Adds each thread's 8 sums over the block's row slots, in order; slot 0 is left with the total.
+__device__ __forceinline__ void slot_sum(f2* f, float* buf, int t, int slot, int slots, int tpr) {
   if (slots == 1) return;
+  f2* at = reinterpret_cast<f2*>(buf);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kGnVals; ++i) buf[(slot * kGnVals + i) * tpr + t] = f[i];
+  for (int i = 0; i < 4; ++i) at[(slot * 4 + i) * tpr + t] = f[i];
   __syncthreads();
   if (slot == 0)
     for (int s = 1; s < slots; ++s)
 #pragma unroll
-      for (int i = 0; i < kGnVals; ++i) f[i] += buf[(s * kGnVals + i) * tpr + t];
+      for (int i = 0; i < 4; ++i) f[i] = f2_add(f[i], at[(s * 4 + i) * tpr + t]);
 }
 
-// Block b takes group b / splits, share b % splits of its rows, then on by the grid.
+template <int VEC>
+__device__ __forceinline__ void gn_part(float* p, const f2* v, int t, int tpr, int C) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[2];
+    f2_unpack(v[i], f[0], f[1]);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int c = gn_channel<VEC>(t, tpr, 2 * i + j);
+      if (c < C) p[c] = f[j];
+    }
+  }
+}
+
+// Block b takes group b / splits, share b % splits of its rows, then on by the grid. The weights
+// wait in shared memory (a thread's 20 pairs of sums take the registers).
 template <typename T, int VEC, int THREADS>
-__global__ void __launch_bounds__(THREADS) gnorm_backward_kernel(GnormArgs a) {
+__global__ void __launch_bounds__(THREADS, THREADS == 128 && VEC > 1 ? 4 : 1) gnorm_backward_kernel(GnormArgs a) {
   constexpr bool MULTI = THREADS > 128;
   __shared__ float red[MULTI ? 128 : 1];
-  extern __shared__ float buf[];
+  extern __shared__ float buf[];  // weights [4][4][tpr] pairs, then the row slots' sums
   int turn = 0;
   const int tpr = a.tpr, t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = blockDim.x / tpr, C = a.C;
   const float inv = 1.f / C;
-  float pw[kGnVals], pb[kGnVals], sc[kGnVals], nw[kGnVals];
-  gn_weight<T, VEC>(a.post_w, a.w_io, t, tpr, C, 1.f, pw);
-  gn_weight<T, VEC>(a.post_b, a.w_io, t, tpr, C, 0.f, pb);
-  gn_weight<T, VEC>(a.res_s, a.w_io, t, tpr, C, 1.f, sc);
-  gn_weight<T, VEC>(a.pre_w, a.w_io, t, tpr, C, 1.f, nw);
-  float apw[kGnVals] = {}, apb[kGnVals] = {}, asc[kGnVals] = {}, anw[kGnVals] = {}, anb[kGnVals] = {};
+  f2* wts = reinterpret_cast<f2*>(buf);
+  if (slot == 0) {
+    f2 w[4];
+    const void* const from[4] = {a.post_w, a.post_b, a.res_s, a.pre_w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      gn_weight<T, VEC>(from[k], a.w_io, t, tpr, C, k == 1 ? 0.f : 1.f, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) wts[(k * 4 + i) * tpr + t] = w[i];
+    }
+  }
+  __syncthreads();
+  auto weight = [&](int k, int i) { return wts[(k * 4 + i) * tpr + t]; };
+  float* sums = buf + 32 * tpr;
+  f2 apw[4] = {}, apb[4] = {}, asc[4] = {}, anw[4] = {}, anb[4] = {};
   const int share = blockIdx.x % a.splits;
+  const int64_t step = static_cast<int64_t>(a.splits) * slots;
   for (int64_t grp = blockIdx.x / a.splits; grp < a.groups; grp += gridDim.x / a.splits) {
-    float ag[kGnVals] = {};
+    f2 ag[4] = {};
     const int64_t end = (grp + 1) * a.group_rows;
-    const int64_t step = static_cast<int64_t>(a.splits) * slots;
-    for (int64_t r0 = grp * a.group_rows + share * slots; r0 < end; r0 += step) {
-      const bool live = r0 + slot < end;
-      const int64_t r = live ? r0 + slot : end - 1;
-      float x[kGnVals], y[kGnVals], g[kGnVals], dh[kGnVals], dn[kGnVals];
-      gn_load<T, VEC>(static_cast<const T*>(a.x) + r * a.xs, t, tpr, C, x);
-      gn_load<T, VEC>(static_cast<const T*>(a.y) + r * a.ys, t, tpr, C, y);
-      if (a.gate) gn_load<T, VEC>(static_cast<const T*>(a.gate) + (a.shared ? grp : r) * a.gs, t, tpr, C, g);
+    GnRaw<T, VEC> rx, ry, rg, rh, rn;
+    float4 st_next;
+    auto load = [&](int64_t r) {
+      r = r < end ? r : end - 1;
+      rx.load(static_cast<const T*>(a.x) + r * a.xs, t, tpr, C);
+      ry.load(static_cast<const T*>(a.y) + r * a.ys, t, tpr, C);
+      if (a.gate) rg.load(static_cast<const T*>(a.gate) + (a.shared ? grp : r) * a.gs, t, tpr, C);
+      if (a.dh) rh.load(static_cast<const T*>(a.dh) + r * a.dhs, t, tpr, C);
+      if (a.dn) rn.load(static_cast<const T*>(a.dn) + r * a.dns, t, tpr, C);
+      st_next = reinterpret_cast<const float4*>(a.stats)[r];
+    };
+    int64_t r0 = grp * a.group_rows + share * slots;
+    if (r0 < end) load(r0 + slot);
+    for (; r0 < end; r0 += step) {
+      const int64_t r = r0 + slot;
+      const bool live = r < end;  // without a row: zero gradients, which add nothing to a sum
+      f2 x[4], y[4], g[4], dh[4] = {}, dn[4] = {};
+      rx.get(x);
+      ry.get(y);
+      if (a.gate) rg.get(g);
+      if (a.dh && live) rh.get(dh);
+      if (a.dn && live) rn.get(dn);
+      const float4 st = st_next;
+      if (r0 + step < end) load(r + step);
+      float s[2];
+      f2 s1 = 0, s2 = 0;
+      // y: normalised y; g: its sigmoid; x: normalised h; dn: d n * pre weight
 #pragma unroll
-      for (int i = 0; i < kGnVals; ++i) dh[i] = dn[i] = 0.f;
-      if (a.dh) gn_load<T, VEC>(static_cast<const T*>(a.dh) + r * a.dhs, t, tpr, C, dh);
-      if (a.dn) gn_load<T, VEC>(static_cast<const T*>(a.dn) + r * a.dns, t, tpr, C, dn);
-      const float4 st = reinterpret_cast<const float4*>(a.stats)[r];
-      const float keep = live ? 1.f : 0.f;
-      float s1 = 0.f, s2 = 0.f;
-      // y: normalised y; g: sigmoid; x: normalised h; dn: d n * pre weight
-#pragma unroll
-      for (int i = 0; i < kGnVals; ++i) {
-        const bool in = gn_channel<VEC>(t, tpr, i) < C;
-        if (a.has_post) y[i] = in ? (y[i] - st.x) * st.y : 0.f;
-        g[i] = a.gate ? gn_sigmoid<T>(g[i]) : 1.f;
+      for (int i = 0; i < 4; ++i) {
+        if (a.has_post) y[i] = f2_mul(f2_add(y[i], f2_both(-st.x)), f2_both(st.y));
+        if (a.gate) g[i] = gn_sigmoid2<T>(g[i]);
         if (a.has_pre) {
-          const float u = a.has_post ? fmaf(y[i], pw[i], pb[i]) : y[i];
-          const float h = fmaf(sc[i], u * g[i], x[i]);
-          x[i] = in ? (h - st.z) * st.w : 0.f;
-          anw[i] = fmaf(keep * dn[i], x[i], anw[i]);
-          anb[i] = fmaf(keep, dn[i], anb[i]);
-          dn[i] *= nw[i];
-          s1 = fmaf(dn[i], x[i], s1);
-          s2 += dn[i];
+          f2 u = a.has_post ? f2_fma(y[i], weight(0, i), weight(1, i)) : y[i];
+          if (a.gate) u = f2_mul(u, g[i]);
+          x[i] = f2_mul(f2_add(f2_fma(weight(2, i), u, x[i]), f2_both(-st.z)), f2_both(st.w));
+          anw[i] = f2_fma(dn[i], x[i], anw[i]);
+          anb[i] = f2_add(dn[i], anb[i]);
+          dn[i] = f2_mul(dn[i], weight(3, i));
+          s1 = f2_fma(dn[i], x[i], s1);
+          s2 = f2_add(dn[i], s2);
         }
       }
       if (a.has_pre) {
-        const float2 s = row_sum<MULTI>(s1, s2, tpr, red, turn);
-        const float m1 = s.x * inv, m2 = a.layer ? s.y * inv : 0.f;
+        s[0] = f2_sum(s1), s[1] = f2_sum(s2);
+        row_sum<MULTI, 2>(s, tpr, red, turn);
+        const f2 m1 = f2_both(-s[0] * inv), m2 = f2_both(a.layer ? -s[1] * inv : 0.f), q = f2_both(st.w);
 #pragma unroll
-        for (int i = 0; i < kGnVals; ++i) dh[i] = fmaf(st.w, dn[i] - x[i] * m1 - m2, dh[i]);
+        for (int i = 0; i < 4; ++i) dh[i] = f2_fma(q, f2_add(f2_fma(x[i], m1, dn[i]), m2), dh[i]);
       }
       if (live) gn_store<T, VEC>(static_cast<T*>(a.dx) + r * C, t, tpr, C, dh);
-      s1 = s2 = 0.f;
-      // dh: d y^ ; dn: d gate
+      s1 = s2 = 0;
+      // dh: d y^; dn: d gate
 #pragma unroll
-      for (int i = 0; i < kGnVals; ++i) {
-        const float u = a.has_post ? fmaf(y[i], pw[i], pb[i]) : y[i];
-        asc[i] = fmaf(keep * dh[i], u * g[i], asc[i]);
-        const float dr = dh[i] * sc[i];
-        dn[i] = dr * u * g[i] * (1.f - g[i]);
-        ag[i] = fmaf(keep, dn[i], ag[i]);
-        const float du = dr * g[i];
-        if (a.has_post) {
-          apw[i] = fmaf(keep * du, y[i], apw[i]);
-          apb[i] = fmaf(keep, du, apb[i]);
+      for (int i = 0; i < 4; ++i) {
+        const f2 u = a.has_post ? f2_fma(y[i], weight(0, i), weight(1, i)) : y[i];
+        f2 dr = dh[i];
+        if (a.gate) {
+          const f2 ug = f2_mul(u, g[i]);
+          asc[i] = f2_fma(dr, ug, asc[i]);
+          dr = f2_mul(dr, weight(2, i));
+          // u sg (1 - sg)
+          dn[i] = f2_mul(dr, f2_fma(f2_mul(ug, g[i]), f2_both(-1.f), ug));
+          ag[i] = f2_add(dn[i], ag[i]);
+          dr = f2_mul(dr, g[i]);
+        } else {
+          asc[i] = f2_fma(dr, u, asc[i]);
+          dr = f2_mul(dr, weight(2, i));
         }
-        dh[i] = a.has_post ? du * pw[i] : du;
-        if (gn_channel<VEC>(t, tpr, i) >= C) dh[i] = 0.f;
-        s1 = fmaf(dh[i], y[i], s1);
-        s2 += dh[i];
+        if (a.has_post) {
+          apw[i] = f2_fma(dr, y[i], apw[i]);
+          apb[i] = f2_add(dr, apb[i]);
+          dr = f2_mul(dr, weight(0, i));
+          s1 = f2_fma(dr, y[i], s1);
+          s2 = f2_add(dr, s2);
+        }
+        dh[i] = dr;
       }
       if (live && a.gate && !a.shared) gn_store<T, VEC>(static_cast<T*>(a.dgate) + r * C, t, tpr, C, dn);
       if (a.has_post) {
-        const float2 s = row_sum<MULTI>(s1, s2, tpr, red, turn);
-        const float m1 = s.x * inv, m2 = a.layer ? s.y * inv : 0.f;
+        s[0] = f2_sum(s1), s[1] = f2_sum(s2);
+        row_sum<MULTI, 2>(s, tpr, red, turn);
+        const f2 m1 = f2_both(-s[0] * inv), m2 = f2_both(a.layer ? -s[1] * inv : 0.f), q = f2_both(st.y);
 #pragma unroll
-        for (int i = 0; i < kGnVals; ++i) dh[i] = st.y * (dh[i] - y[i] * m1 - m2);
+        for (int i = 0; i < 4; ++i) dh[i] = f2_mul(q, f2_add(f2_fma(y[i], m1, dh[i]), m2));
       }
       if (live) gn_store<T, VEC>(static_cast<T*>(a.dy) + r * C, t, tpr, C, dh);
     }
     if (a.shared) {
-      slot_sum<VEC>(ag, buf, t, slot, slots, tpr);
+      slot_sum(ag, sums, t, slot, slots, tpr);
       if (slot == 0) {
-        if (a.gpart) {
-          float* p = a.gpart + (grp * a.splits + share) * C;
-#pragma unroll
-          for (int i = 0; i < kGnVals; ++i) {
-            const int c = gn_channel<VEC>(t, tpr, i);
-            if (c < C) p[c] = ag[i];
-          }
-        } else {
+        if (a.gpart)
+          gn_part<VEC>(a.gpart + (grp * a.splits + share) * C, ag, t, tpr, C);
+        else
           gn_store<T, VEC>(static_cast<T*>(a.dgate) + grp * C, t, tpr, C, ag);
-        }
       }
     }
   }
-  float* const acc[5] = {apw, apb, asc, anw, anb};
-#pragma unroll
-  for (int k = 0; k < 5; ++k) {
-    slot_sum<VEC>(acc[k], buf, t, slot, slots, tpr);
-    if (slot == 0) {
-      float* p = a.part + (static_cast<int64_t>(blockIdx.x) * 5 + k) * C;
-#pragma unroll
-      for (int i = 0; i < kGnVals; ++i) {
-        const int c = gn_channel<VEC>(t, tpr, i);
-        if (c < C) p[c] = acc[k][i];
-      }
-    }
-  }
+  float* part = a.part + static_cast<int64_t>(blockIdx.x) * 5 * C;
+  auto leave = [&](f2* v, int k) {
+    slot_sum(v, sums, t, slot, slots, tpr);
+    if (slot == 0) gn_part<VEC>(part + k * C, v, t, tpr, C);
+  };
+  leave(apw, 0);
+  leave(apb, 1);
+  leave(asc, 2);
+  leave(anw, 3);
+  leave(anb, 4);
 }
 
 // out[set][c] = sum over n of in[(set_base + n * set_step) ...]: the blocks' partial rows, added
@@ -404,7 +481,7 @@ inline GnormPlan gnorm_plan(int64_t rows, int64_t gate_rows, int64_t C) {
   p.threads = p.tpr <= 32 ? 128 : p.tpr;
   p.slots = p.threads / p.tpr;
   const int64_t sms = sm_count();
-  const int64_t most = sms * (p.threads <= 128 ? 8 : p.threads <= 256 ? 4 : 2);
+  const int64_t most = sms * (p.threads <= 128 ? 5 : p.threads <= 256 ? 3 : 2);
   const int64_t need = (rows + p.slots - 1) / p.slots;
   p.blocks = need < most ? need : most;
   const int64_t bmost = sms * (p.threads <= 128 ? 4 : p.threads <= 256 ? 2 : 1);
@@ -513,10 +590,11 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
                     aligned16(y) && aligned16(gate) && aligned16(dh) && aligned16(dn) && aligned16(dx) &&
                     aligned16(dy) && aligned16(dgate);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const size_t smem = p.slots > 1 ? static_cast<size_t>(p.threads) * kGnVals * 4 : 0;
+  const size_t smem = static_cast<size_t>(p.tpr) * 128 + (p.slots > 1 ? static_cast<size_t>(p.threads) * kGnVals * 4 : 0);
   int rc = gnorm_dispatch(dtype, fits, p.tpr, [&](auto t, auto v, auto m) {
-    gnorm_backward_kernel<decltype(t), decltype(v)::value, decltype(m)::value>
-        <<<static_cast<unsigned>(p.bblocks), p.threads, smem, st>>>(a);
+    auto kern = gnorm_backward_kernel<decltype(t), decltype(v)::value, decltype(m)::value>;
+    if (smem > 48 * 1024) set_smem(kern, smem);
+    kern<<<static_cast<unsigned>(p.bblocks), p.threads, smem, st>>>(a);
     return launch_status();
   });
   if (rc != TOPS_OK) return rc;

@@ -19,6 +19,7 @@ struct RotaryArgs {
   int64_t B, N;
   int Hq, Hk, D, P, A;  // P pairs, 2 P <= D; A axes
   int interleaved, wide, negate;  // wide: int64 positions
+  int tok;                        // tokens a block
   const void *q, *k;
   int64_t qs[3], ks[3], ps[3];  // strides of (batch, token, head) and of positions (axis, batch, token)
   const void* pos;
@@ -28,7 +29,6 @@ struct RotaryArgs {
 };
 
 constexpr int kRotThreads = 256;
-constexpr int kRotTokens = 4;
 
 __device__ __forceinline__ float2 turn_of(double pos, float freq) {
   const double a = pos * freq;
@@ -38,46 +38,90 @@ __device__ __forceinline__ float2 turn_of(double pos, float freq) {
   return make_float2(c, s);
 }
 
-template <typename T>
+// VEC channels of one head at a time as 16 bytes (VEC 1: one by one): the two halves' channels of
+// VEC pairs, or VEC / 2 neighbouring pairs. Block (x, y): tokens x * tok.., share y of the heads.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
-  extern __shared__ float2 cs[];  // [kRotTokens][P]
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kRotTokens, tokens = a.B * a.N;
-  const int nt = static_cast<int>(tokens - t0 < kRotTokens ? tokens - t0 : kRotTokens);
-  for (int i = threadIdx.x; i < nt * a.P; i += kRotThreads) {
-    const int64_t tok = t0 + i / a.P;
-    const int f = i % a.P;
+  extern __shared__ float2 cs[];  // [tok][P]
+  const uint32_t t0 = blockIdx.x * a.tok, tokens = static_cast<uint32_t>(a.B * a.N), N = static_cast<uint32_t>(a.N);
+  const uint32_t nt = min(static_cast<uint32_t>(a.tok), tokens - t0), P = a.P;
+  for (uint32_t i = threadIdx.x; i < nt * P; i += kRotThreads) {
+    const uint32_t tok = t0 + i / P, f = i % P;
     const int ax = a.axis[f];
-    if (ax < 0 || ax >= a.A) {  // no such axis: the pair stays as it is
-      cs[i] = make_float2(1.f, 0.f);
-      continue;
+    float2 v = make_float2(1.f, 0.f);  // no such axis: the pair stays as it is
+    if (ax >= 0 && ax < a.A) {
+      const int64_t at = ax * a.ps[0] + tok / N * a.ps[1] + tok % N * a.ps[2];
+      const double p = a.wide ? static_cast<double>(static_cast<const int64_t*>(a.pos)[at])
+                              : static_cast<double>(static_cast<const int*>(a.pos)[at]);
+      v = turn_of(p, a.inv_freq[f]);
+      if (a.negate) v.y = -v.y;
     }
-    const int64_t at = ax * a.ps[0] + tok / a.N * a.ps[1] + tok % a.N * a.ps[2];
-    const double p = a.wide ? static_cast<double>(static_cast<const int64_t*>(a.pos)[at])
-                            : static_cast<double>(static_cast<const int*>(a.pos)[at]);
-    float2 v = turn_of(p, a.inv_freq[f]);
-    if (a.negate) v.y = -v.y;
     cs[i] = v;
   }
   __syncthreads();
-  const int H = a.Hq + a.Hk, half = a.D / 2;
-  for (int i = threadIdx.x; i < nt * H * a.D; i += kRotThreads) {
-    const int d = i % a.D, h = i / a.D % H, ti = i / a.D / H;
-    const int64_t tok = t0 + ti, b = tok / a.N, n = tok % a.N;
-    const bool isq = h < a.Hq;
-    const int hh = isq ? h : h - a.Hq;
+  const uint32_t H = a.Hq + a.Hk, half = a.D / 2;
+  const uint32_t h_lo = H * blockIdx.y / gridDim.y, nh = H * (blockIdx.y + 1) / gridDim.y - h_lo;
+  // items of a head: pieces of the first half with their mates in the second, and (odd D) the last
+  // channel; or pieces of neighbouring pairs
+  const uint32_t items = a.interleaved ? (a.D + VEC - 1) / VEC : VEC == 1 ? a.D - half : half / VEC;
+  for (uint32_t i = threadIdx.x; i < nt * nh * items; i += kRotThreads) {
+    const uint32_t hi = i / items, e = i % items, ti = hi / nh, h = h_lo + hi % nh;
+    const uint32_t tok = t0 + ti, b = tok / N, n = tok % N;
+    const bool isq = h < static_cast<uint32_t>(a.Hq);
+    const uint32_t hh = isq ? h : h - a.Hq;
     const T* src = isq ? static_cast<const T*>(a.q) + b * a.qs[0] + n * a.qs[1] + hh * a.qs[2]
                        : static_cast<const T*>(a.k) + b * a.ks[0] + n * a.ks[1] + hh * a.ks[2];
-    T* dst = isq ? static_cast<T*>(a.qo) + (tok * a.Hq + hh) * a.D : static_cast<T*>(a.ko) + (tok * a.Hk + hh) * a.D;
-    const int f = a.interleaved ? d / 2 : d % half;
-    const bool second = a.interleaved ? d & 1 : d >= half;
-    if (f >= a.P || (!a.interleaved && d >= 2 * half)) {
-      dst[d] = src[d];
-      continue;
+    T* dst = isq ? static_cast<T*>(a.qo) + (static_cast<int64_t>(tok) * a.Hq + hh) * a.D
+                 : static_cast<T*>(a.ko) + (static_cast<int64_t>(tok) * a.Hk + hh) * a.D;
+    const float2* w = cs + ti * P;
+    if constexpr (VEC == 1) {
+      const uint32_t f = a.interleaved ? e / 2 : e;
+      const uint32_t d = e, mate = a.interleaved ? e ^ 1 : e + half;
+      if (a.interleaved) {
+        if (f >= P) {
+          dst[d] = src[d];
+        } else {
+          const float u = static_cast<float>(src[d]), v = static_cast<float>(src[mate]);
+          dst[d] = static_cast<T>(e & 1 ? fmaf(u, w[f].x, v * w[f].y) : fmaf(u, w[f].x, -(v * w[f].y)));
+        }
+      } else if (f >= P) {
+        if (f < half) dst[d] = src[d];
+        dst[mate] = src[mate];
+      } else {
+        const float u = static_cast<float>(src[d]), v = static_cast<float>(src[mate]);
+        dst[d] = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
+        dst[mate] = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
+      }
+    } else {
+      union Piece {
+        uint4 w;
+        T v[VEC];
+      };
+      Piece p, r;
+      p.w = *reinterpret_cast<const uint4*>(src + e * VEC);
+      if (a.interleaved) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 2) {
+          const uint32_t f = (e * VEC + j) / 2;
+          if (f >= P) continue;
+          const float u = static_cast<float>(p.v[j]), v = static_cast<float>(p.v[j + 1]);
+          p.v[j] = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
+          p.v[j + 1] = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
+        }
+      } else {
+        r.w = *reinterpret_cast<const uint4*>(src + half + e * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const uint32_t f = e * VEC + j;
+          if (f >= P) continue;
+          const float u = static_cast<float>(p.v[j]), v = static_cast<float>(r.v[j]);
+          p.v[j] = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
+          r.v[j] = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
+        }
+        *reinterpret_cast<uint4*>(dst + half + e * VEC) = r.w;
+      }
+      *reinterpret_cast<uint4*>(dst + e * VEC) = p.w;
     }
-    const int mate = a.interleaved ? d ^ 1 : second ? d - half : d + half;
-    const float2 w = cs[ti * a.P + f];
-    const float u = static_cast<float>(src[d]), v = static_cast<float>(src[mate]);
-    dst[d] = static_cast<T>(second ? fmaf(u, w.x, v * w.y) : fmaf(u, w.x, -(v * w.y)));
   }
 }
 
@@ -103,10 +147,25 @@ extern "C" int tops_rotary(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t 
   a.q = q, a.k = k, a.pos = positions, a.inv_freq = inv_freq, a.axis = axis, a.qo = q_out, a.ko = k_out;
   for (int i = 0; i < 3; ++i) a.qs[i] = strides[i], a.ks[i] = strides[3 + i], a.ps[i] = pos_strides[i];
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const unsigned grid = static_cast<unsigned>((B * N + kRotTokens - 1) / kRotTokens);
-  const size_t smem = kRotTokens * P * sizeof(float2);
+  // few tokens: one a block, and the heads shared by blocks until the SMs are busy
+  const int64_t tokens = B * N, sms = sm_count();
+  a.tok = tokens >= 8 * sms ? 4 : 1;
+  const int64_t blocks = (tokens + a.tok - 1) / a.tok;
+  int64_t shares = tokens >= 8 * sms ? 1 : (2 * sms + blocks - 1) / blocks;
+  shares = shares < Hq + Hk ? shares : Hq + Hk;
+  const size_t smem = a.tok * P * sizeof(float2);
   return by_io_type(dtype, [&](auto t) {
-    rotary_kernel<decltype(t)><<<grid, kRotThreads, smem, st>>>(a);
+    using T = decltype(t);
+    constexpr int VEC = 16 / sizeof(T);
+    auto fits = [&](const void* p, const void* o, const int64_t* st) {
+      return aligned16(p) && aligned16(o) && st[0] % VEC == 0 && st[1] % VEC == 0 && st[2] % VEC == 0;
+    };
+    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(shares));
+    if (D % (interleaved ? VEC : 2 * VEC) == 0 && (Hq == 0 || fits(q, q_out, a.qs)) &&
+        (Hk == 0 || fits(k, k_out, a.ks)))
+      rotary_kernel<T, VEC><<<grid, kRotThreads, smem, st>>>(a);
+    else
+      rotary_kernel<T, 1><<<grid, kRotThreads, smem, st>>>(a);
     return launch_status();
   });
 }

@@ -33,7 +33,8 @@ _lib.register("tops_window_attn_backward",
 _lib.register("tops_window_attn_backward_workspace_bytes",
               [_I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P])
 _lib.register("tops_window_attn_decode",
-              [_I, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _F, _P, _P])
+              [_I, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _P, _I64, _I64, _F, _P, _P, _P])
+_lib.register("tops_window_attn_decode_workspace_bytes", [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _P])
 
 
 def _window(window):
@@ -162,8 +163,12 @@ def decode(q, k_cache, v_cache, lengths, *, window, sinks=0, scale=None):
     q, k, v = _rows(q), _rows(k_cache), _rows(v_cache)
     lengths = lengths.to(torch.int32).contiguous()
     out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    need = ctypes.c_int64(0)
+    _lib.call("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, window, int(sinks), ctypes.byref(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     with torch.cuda.device(q.device):
         _lib.call("tops_window_attn_decode", dt, B, N, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   _strides(q, k, v), lengths.data_ptr(), window, int(sinks),
-                  D ** -0.5 if scale is None else float(scale), out.data_ptr(), _lib.stream_ptr(q.device))
+                  D ** -0.5 if scale is None else float(scale), _lib.ptr(ws), out.data_ptr(),
+                  _lib.stream_ptr(q.device))
     return out
