@@ -99,6 +99,25 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
+_FN: dict = {}
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call an entry point whose last argument is the stream, on ``device`` and its current
+    stream. The checks and look-ups of :func:`call`, at the cost that a single token allows."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(lib(), name)
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(device):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code != OK:
+        check(code, name)
+
+
 def dtype_code(dtype: torch.dtype) -> int:
     try:
         return _DTYPE_CODE[dtype]

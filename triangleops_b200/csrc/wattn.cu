@@ -120,7 +120,10 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     sm.abort = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(&sm.tmem_base, 256);
+  if (warp == 1) {
+    tmem_alloc(&sm.tmem_base, 256);
+    tmem_relinquish();  // the SM's other CTA allocates too
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();

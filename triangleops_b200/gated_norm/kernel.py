@@ -39,16 +39,21 @@ def _rows(t, C):
     the tensor has no such view)."""
     if t is None:
         return None
+    if t.is_contiguous():
+        return t
     if t.dim() == 2 and t.stride(1) == 1:
         return t
-    if t.is_contiguous():
-        return t.view(-1, C)
     if t.shape[-1] == 1 or t.stride(-1) == 1:
         try:
             return t.view(-1, C)
         except RuntimeError:
             pass
-    return t.contiguous().view(-1, C)
+    return t.contiguous()
+
+
+def _pitch(t, C):
+    """Row stride of what :func:`_rows` gave."""
+    return 0 if t is None else C if t.is_contiguous() else t.stride(0)
 
 
 def _check(x, y, gate, weights, kind):
@@ -73,9 +78,10 @@ def _check(x, y, gate, weights, kind):
     wt = {w.dtype for w in weights if w is not None}
     if len(wt) > 1 or not wt <= {x.dtype, torch.float32}:
         raise ValueError(f"the weights must all be {x.dtype} or all fp32, got {sorted(map(str, wt))}")
+    dev = x.device
     for w in weights:
-        assert w is None or (w.shape == (C,) and w.device == x.device), "a weight must be (C,) on the device of x"
-    assert y.device == x.device and (gate is None or gate.device == x.device), "x, y and gate must be on one device"
+        assert w is None or (w.shape == (C,) and w.device == dev), "a weight must be (C,) on the device of x"
+    assert y.device == dev and (gate is None or gate.device == dev), "x, y and gate must be on one device"
     w_dt = _lib.dtype_code(wt.pop()) if wt else dt
     return dt, w_dt, C, rows, groups
 
@@ -90,18 +96,17 @@ def forward(x, y, gate=None, *, post_weight=None, post_bias=None, res_scale=None
     :func:`backward` (mean and 1/std of y, of h)."""
     weights = [_w(w) for w in (post_weight, post_bias, res_scale, pre_weight, pre_bias)]
     dt, w_dt, C, rows, groups = _check(x, y, gate, weights, kind)
-    _lib.require_cuda(x, y)
+    _lib.require_cuda(x)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     n = torch.empty_like(h) if pre_norm else None
-    stats = torch.empty(*x.shape[:-1], 4, dtype=torch.float32, device=x.device)
+    stats = torch.empty((*x.shape[:-1], 4), dtype=torch.float32, device=x.device)
     if rows == 0:
         return h, n, stats
     x2, y2, g2 = _rows(x, C), _rows(y, C), _rows(gate, C)
-    with torch.cuda.device(x.device):
-        _lib.call("tops_gated_norm_forward", dt, w_dt, rows, groups, C, kind == "layer", bool(post_norm),
-                  bool(pre_norm), float(eps), x2.data_ptr(), x2.stride(0), y2.data_ptr(), y2.stride(0), _lib.ptr(g2),
-                  0 if g2 is None else g2.stride(0), *map(_lib.ptr, weights), h.data_ptr(), _lib.ptr(n),
-                  stats.data_ptr(), _lib.stream_ptr(x.device))
+    ptr = _lib.ptr
+    _lib.launch("tops_gated_norm_forward", x.device, dt, w_dt, rows, groups, C, kind == "layer", bool(post_norm),
+                bool(pre_norm), float(eps), x2.data_ptr(), _pitch(x2, C), y2.data_ptr(), _pitch(y2, C), ptr(g2),
+                _pitch(g2, C), *map(ptr, weights), h.data_ptr(), ptr(n), stats.data_ptr())
     return h, n, stats
 
 
@@ -116,11 +121,13 @@ def backward(dh, dn, x, y, gate, stats, *, post_weight=None, post_bias=None, res
     dt, w_dt, C, rows, groups = _check(x, y, gate, weights, kind)
     for d in (dh, dn):
         assert d is None or d.shape == x.shape, "dh and dn must be like x"
+        assert d is None or d.device == x.device, "dh and dn must be on the device of x"
         if d is not None and d.dtype != x.dtype:
             raise ValueError(f"dh and dn must be {x.dtype}")
     assert stats.shape == (*x.shape[:-1], 4) and stats.dtype == torch.float32 and stats.is_contiguous(), \
         "stats must be what forward returned"
-    _lib.require_cuda(x, y, stats)
+    assert stats.device == x.device, "stats must be on the device of x"
+    _lib.require_cuda(x)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     res = {"dx": dx, "dy": torch.empty_like(dx)}
     if gate is not None:
@@ -137,12 +144,10 @@ def backward(dh, dn, x, y, gate, stats, *, post_weight=None, post_bias=None, res
         _lib.call("tops_gated_norm_backward_workspace_bytes", rows, groups, C, ctypes.byref(need))
         ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
         x2, y2, g2, dh2, dn2 = (_rows(t, C) for t in (x, y, gate, dh, dn))
-        st = [0 if t is None else t.stride(0) for t in (dh2, dn2, x2, y2, g2)]
-        with torch.cuda.device(x.device):
-            _lib.call("tops_gated_norm_backward", dt, w_dt, rows, groups, C, kind == "layer", bool(post_norm),
-                      bool(pre_norm), _lib.ptr(dh2), st[0], _lib.ptr(dn2), st[1], x2.data_ptr(), st[2], y2.data_ptr(),
-                      st[3], _lib.ptr(g2), st[4], stats.data_ptr(), *map(_lib.ptr, weights[:4]), dx.data_ptr(),
-                      res["dy"].data_ptr(), _lib.ptr(res.get("dgate")), *map(_lib.ptr, dw), ws.data_ptr(),
-                      _lib.stream_ptr(x.device))
+        ptr = _lib.ptr
+        _lib.launch("tops_gated_norm_backward", x.device, dt, w_dt, rows, groups, C, kind == "layer", bool(post_norm),
+                    bool(pre_norm), ptr(dh2), _pitch(dh2, C), ptr(dn2), _pitch(dn2, C), x2.data_ptr(), _pitch(x2, C),
+                    y2.data_ptr(), _pitch(y2, C), ptr(g2), _pitch(g2, C), stats.data_ptr(), *map(ptr, weights[:4]),
+                    dx.data_ptr(), res["dy"].data_ptr(), ptr(res.get("dgate")), *map(ptr, dw), ws.data_ptr())
     res.update({"d" + k: w for k, w in zip(named, dw) if w is not None})
     return res

@@ -22,6 +22,8 @@ _P, _I, _I64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64
 _lib.register("tops_rotary",
               [_I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _P])
 
+_I3, _I6 = ctypes.c_int64 * 3, ctypes.c_int64 * 6
+
 
 def _turn(q, k, positions, inv_freq, axis, interleaved, negate):
     dt = _lib.dtype_code(q.dtype)
@@ -42,22 +44,21 @@ def _turn(q, k, positions, inv_freq, axis, interleaved, negate):
         if k.dtype != q.dtype:
             raise ValueError(f"q and k must have one dtype, got {q.dtype} and {k.dtype}")
         Hk = k.shape[2]
-    for t in (k, positions, inv_freq, axis):
-        assert t is None or t.device == q.device, "q, k, positions, inv_freq and axis must be on one device"
+    dev = q.device
+    assert positions.device == inv_freq.device == axis.device == dev and (k is None or k.device == dev), \
+        "q, k, positions, inv_freq and axis must be on one device"
     _lib.require_cuda(q)
-    qo = torch.empty(B, N, Hq, D, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(B, N, Hk, D, dtype=q.dtype, device=q.device)
+    qo = torch.empty((B, N, Hq, D), dtype=q.dtype, device=dev)
+    ko = None if k is None else torch.empty((B, N, Hk, D), dtype=q.dtype, device=dev)
     if q.stride(3) != 1:
         q = q.contiguous()
     if k is not None and k.stride(3) != 1:
         k = k.contiguous()
-    st = (ctypes.c_int64 * 6)(*q.stride()[:3], *(k.stride()[:3] if k is not None else (0, 0, 0)))
-    ps = (ctypes.c_int64 * 3)(*positions.stride())
+    st = _I6(*q.stride()[:3], *(k.stride()[:3] if k is not None else (0, 0, 0)))
     inv_freq, axis = inv_freq.contiguous(), axis.contiguous()
-    with torch.cuda.device(q.device):
-        _lib.call("tops_rotary", dt, B, N, Hq, Hk, D, P, positions.shape[0], bool(interleaved), negate, q.data_ptr(),
-                  _lib.ptr(k), st, positions.data_ptr(), positions.dtype == torch.int64, ps, inv_freq.data_ptr(),
-                  axis.data_ptr(), qo.data_ptr(), _lib.ptr(ko), _lib.stream_ptr(q.device))
+    _lib.launch("tops_rotary", dev, dt, B, N, Hq, Hk, D, P, positions.shape[0], bool(interleaved), negate,
+                q.data_ptr(), _lib.ptr(k), st, positions.data_ptr(), positions.dtype == torch.int64,
+                _I3(*positions.stride()), inv_freq.data_ptr(), axis.data_ptr(), qo.data_ptr(), _lib.ptr(ko))
     return qo, ko
 
 

@@ -58,6 +58,8 @@ def _tiles(t):
     """As :func:`_rows`, and where the tensor cores take the type and head size, with rows that
     their loads can follow: 16-byte aligned, none repeated by a stride of zero (one copy costs
     far less than the CUDA-core path that takes such rows as they are)."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     t = _rows(t)
     if t.dtype == torch.float32 or t.shape[-1] % 8 or t.shape[-1] > 128:
         return t
@@ -66,16 +68,18 @@ def _tiles(t):
     return t
 
 
-def _strides(*tensors):
-    st = [s for t in tensors for s in t.stride()[:-1]]
-    return (ctypes.c_int64 * len(st))(*st)
+_I3, _I8, _I9 = ctypes.c_int64 * 3, ctypes.c_int64 * 8, ctypes.c_int64 * 9
+
+
+def _strides(q, k, v):
+    return _I9(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3])
 
 
 def _check(q, k, v):
     assert q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q, k and v must be (B, N, H, D)"
     B, Nq, Hq, D = q.shape
-    assert k.shape == v.shape and k.shape[0] == B and k.shape[3] == D, "k and v must be (B, Nk, Hkv, D) like q"
-    Nk, Hkv = k.shape[1], k.shape[2]
+    Bk, Nk, Hkv, Dk = k.shape
+    assert k.shape == v.shape and Bk == B and Dk == D, "k and v must be (B, Nk, Hkv, D) like q"
     assert Hkv > 0 and Hq % Hkv == 0, "the query heads must be a multiple of the key heads"
     assert Nk >= Nq, "the queries are the last Nq of the Nk tokens"
     if not (q.dtype == k.dtype == v.dtype):
@@ -91,7 +95,7 @@ def _mask(mask, B, Nk, device):
     assert mask.device == device, "mask must be on the device of q"
     if mask.dtype != torch.bool:
         mask = mask != 0
-    return mask.contiguous().view(torch.uint8)
+    return mask.contiguous()
 
 
 def forward(q, k, v, *, window, sinks=0, scale=None, mask=None, out=None):
@@ -102,17 +106,19 @@ def forward(q, k, v, *, window, sinks=0, scale=None, mask=None, out=None):
     dt = _lib.dtype_code(q.dtype)
     B, Nq, Nk, Hq, Hkv, D = _check(q, k, v)
     left, right = _window(window)
-    _lib.require_cuda(q, k, v)
-    m = _mask(mask, B, Nk, q.device)
+    dev = q.device
+    _lib.require_cuda(q)
+    m = _mask(mask, B, Nk, dev)
     q, k, v = _tiles(q), _tiles(k), _tiles(v)
     if out is None:
-        out = torch.empty(B, Nq, Hq, D, dtype=q.dtype, device=q.device)
-    assert out.shape == (B, Nq, Hq, D) and out.dtype == q.dtype and out.is_contiguous(), "out must be like q, contiguous"
-    lse = torch.empty(B, Hq, Nq, dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("tops_window_attn_forward", dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides(q, k, v), _lib.ptr(m), left, right, int(sinks), D ** -0.5 if scale is None else float(scale),
-                  out.data_ptr(), lse.data_ptr(), _lib.stream_ptr(q.device))
+        out = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=dev)
+    else:
+        assert out.shape == (B, Nq, Hq, D) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev, \
+            "out must be like q, contiguous"
+    lse = torch.empty((B, Hq, Nq), dtype=torch.float32, device=dev)
+    _lib.launch("tops_window_attn_forward", dev, dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                _strides(q, k, v), None if m is None else m.data_ptr(), left, right, int(sinks),
+                D ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr())
     return out, lse
 
 
@@ -127,22 +133,23 @@ def backward(dout, q, k, v, out, lse, *, window, sinks=0, scale=None, mask=None)
     assert lse.shape == (B, Hq, Nq) and lse.dtype == torch.float32, "lse must be (B, Hq, Nq) fp32"
     if dout.dtype != q.dtype or out.dtype != q.dtype:
         raise ValueError(f"dout and out must be {q.dtype}")
-    _lib.require_cuda(q, k, v, dout, out, lse)
-    m = _mask(mask, B, Nk, q.device)
+    dev = q.device
+    assert dout.device == out.device == lse.device == dev, "dout, out and lse must be on the device of q"
+    _lib.require_cuda(q)
+    m = _mask(mask, B, Nk, dev)
     q, k, v, dout = _tiles(q), _tiles(k), _tiles(v), _tiles(dout)
     out, lse = out.contiguous(), lse.contiguous()
-    dq = torch.empty(B, Nq, Hq, D, dtype=q.dtype, device=q.device)
-    dk = torch.empty(B, Nk, Hkv, D, dtype=q.dtype, device=q.device)
+    dq = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=dev)
+    dk = torch.empty((B, Nk, Hkv, D), dtype=q.dtype, device=dev)
     dv = torch.empty_like(dk)
     need = ctypes.c_int64(0)
     _lib.call("tops_window_attn_backward_workspace_bytes", dt, B, Nq, Nk, Hq, Hkv, D, left, right, int(sinks),
               ctypes.byref(need))
-    ws = torch.empty(max(16, need.value), dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("tops_window_attn_backward", dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides(q, k, v), _lib.ptr(m), left, right, int(sinks), D ** -0.5 if scale is None else float(scale),
-                  dout.data_ptr(), _strides(dout), out.data_ptr(), lse.data_ptr(), ws.data_ptr(), dq.data_ptr(),
-                  dk.data_ptr(), dv.data_ptr(), _lib.stream_ptr(q.device))
+    ws = torch.empty(max(16, need.value), dtype=torch.uint8, device=dev)
+    _lib.launch("tops_window_attn_backward", dev, dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                _strides(q, k, v), None if m is None else m.data_ptr(), left, right, int(sinks),
+                D ** -0.5 if scale is None else float(scale), dout.data_ptr(), _I3(*dout.stride()[:3]),
+                out.data_ptr(), lse.data_ptr(), ws.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr())
     return dq, dk, dv
 
 
@@ -153,22 +160,28 @@ def decode(q, k_cache, v_cache, lengths, *, window, sinks=0, scale=None):
     device; a length of 0 gives zeros, one beyond N counts as N. Returns (B, Hq, D)."""
     dt = _lib.dtype_code(q.dtype)
     assert q.dim() == 3, "q must be (B, Hq, D)"
+    assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape, "the caches must be (B, N, Hkv, D)"
     B, Hq, D = q.shape
-    _check(q.unsqueeze(1), k_cache, v_cache)
-    N, Hkv = k_cache.shape[1], k_cache.shape[2]
-    assert lengths.shape == (B,) and lengths.device == q.device, "lengths must be (B,) on the device of q"
+    Bk, N, Hkv, Dk = k_cache.shape
+    assert Bk == B and Dk == D, "the caches must be (B, N, Hkv, D) like q"
+    assert Hkv > 0 and Hq % Hkv == 0, "the query heads must be a multiple of the key heads"
+    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+        raise ValueError(f"q and the caches must have one dtype, got {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    dev = q.device
+    assert k_cache.device == v_cache.device == lengths.device == dev, "q, the caches and lengths must be on one device"
+    assert lengths.shape == (B,), "lengths must be (B,)"
     if not isinstance(window, int) or window < 1:
         raise ValueError(f"window must be a number of keys, at least 1, got {window}")
-    _lib.require_cuda(q, k_cache, v_cache, lengths)
+    _lib.require_cuda(q)
+    sinks = int(sinks)
     q, k, v = _rows(q), _rows(k_cache), _rows(v_cache)
-    lengths = lengths.to(torch.int32).contiguous()
-    out = torch.empty(B, Hq, D, dtype=q.dtype, device=q.device)
+    if lengths.dtype != torch.int32 or not lengths.is_contiguous():
+        lengths = lengths.to(torch.int32).contiguous()
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
     need = ctypes.c_int64(0)
-    _lib.call("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, window, int(sinks), ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-    with torch.cuda.device(q.device):
-        _lib.call("tops_window_attn_decode", dt, B, N, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-                  _strides(q, k, v), lengths.data_ptr(), window, int(sinks),
-                  D ** -0.5 if scale is None else float(scale), _lib.ptr(ws), out.data_ptr(),
-                  _lib.stream_ptr(q.device))
+    _lib.call("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, window, sinks, ctypes.byref(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=dev).data_ptr() if need.value else None
+    _lib.launch("tops_window_attn_decode", dev, dt, B, N, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                _I8(*q.stride()[:2], *k.stride()[:3], *v.stride()[:3]), lengths.data_ptr(), window, sinks,
+                D ** -0.5 if scale is None else float(scale), ws, out.data_ptr())
     return out
