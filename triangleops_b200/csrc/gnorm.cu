@@ -47,7 +47,6 @@ struct GnormArgs {
 };
 
 constexpr int kGnVals = 8;  // channels per thread, held as 4 pairs (packed fp32 arithmetic)
-using f2 = unsigned long long;
 
 // channel of value i (0..7) of the thread at `t` of a row of tpr threads
 template <int VEC>
@@ -133,7 +132,6 @@ __device__ __forceinline__ void gn_weight(const void* w, int io, int t, int tpr,
   for (int i = 0; i < 4; ++i) f[i] = f2_pack(v[2 * i], v[2 * i + 1]);
 }
 
-__device__ __forceinline__ f2 f2_both(float x) { return f2_pack(x, x); }
 __device__ __forceinline__ float f2_sum(f2 v) {
   float a, b;
   f2_unpack(v, a, b);

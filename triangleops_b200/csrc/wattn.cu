@@ -4,20 +4,20 @@
 //   S = q k^T,  P = 2^(c (S - m)) with c = scale log2(e),  O = P v / sum P,  lse = ln2 (c m + log2 sum P)
 // over the keys that a query sees (wattn.h), in one walk over them with a running maximum m and sum.
 //
-// A block (CTA) takes 128 queries of one head and walks over 128-key blocks: the sinks, where the
+// A block (CTA) takes 128 queries of one head and walks over 64-key blocks: the sinks, where the
 // window has left them behind, then the window, which starts exactly at the first key that the
 // tile's first query sees (a TMA row coordinate needs no alignment), so a window of W costs
-// ceil((W + 127) / 128) blocks. Only blocks on the edge of the window, or with a masked key, test
+// ceil((W + 127) / 64) blocks. Only blocks on the edge of the window, or with a masked key, test
 // their keys; the others run without. Up to 32 left-behind sinks are a block of 32 keys.
 //
-// One warp loads (TMA; keys past the end and channels past D arrive as zeros), one issues the
-// MMAs, four hold the softmax: a thread owns a query row (a TMEM lane), so row maximum and sum need
-// no exchange. S is a fp32 TMEM tile, P goes back to TMEM rounded to the IO dtype (the product's
+// One warp loads (TMA; keys past the end and channels past D arrive as zeros), one issues the MMAs
+// of S and another those of P v (a thread takes some 85 cycles to issue one of them, and 100 for a
+// commit: one thread for both took 1.9 k cycles a block and was what bound the kernel), four hold
+// the softmax: a thread owns a query row (a TMEM lane), so row maximum and sum need
+// no exchange. S is a fp32 TMEM tile, P takes its place rounded to the IO dtype (the product's
 // operand type; its sum is taken before the rounding), O accumulates in TMEM and is rescaled only
-// when the maximum has grown by 2^8. Two CTAs share an SM and its 512 TMEM columns, so that one's
-// MMAs run under the other's softmax. D > 64: P takes S's columns and S of the next block follows
-// P v of this one; D <= 64: P has its own columns and S of the next block is computed under the
-// softmax of this one.
+// when the maximum has grown by 2^8. S has two buffers: q k^T of the next block runs under the
+// softmax of this one. Two CTAs share an SM and its 512 TMEM columns (S 2 x 64, O up to 128 each).
 //
 // Masked keys: their score is replaced by -inf, and their rows of the V tile are zeroed in shared
 // memory before P v, so that a NaN there does not pass through 0 * NaN.
@@ -37,24 +37,23 @@ struct WattnFwdArgs {
 
 template <int DT>
 struct WattnFwdCfg {
-  static constexpr int SUB = DT / 64;             // 64-channel sub-tiles (128-byte rows, 128B swizzle)
-  static constexpr int TILE = SUB * 128 * 128;    // bytes of a 128-row tile
-  static constexpr int NS = DT == 128 ? 1 : 2;    // K and V stages
-  static constexpr int S_COL = 0;
-  static constexpr int P_COL = DT == 128 ? 0 : 128;
-  static constexpr int O_COL = DT == 128 ? 128 : 192;
-  static constexpr bool AHEAD = P_COL != S_COL;   // S of the next block before P v of this one
-  static constexpr int THREADS = 192;
+  static constexpr int SUB = DT / 64;            // 64-channel sub-tiles (128-byte rows, 128B swizzle)
+  static constexpr int BK = 64;                  // keys a block
+  static constexpr int Q_TILE = SUB * 128 * 128;
+  static constexpr int TILE = SUB * BK * 128;    // bytes of a K or V tile
+  static constexpr int NS = 2;                   // K and V stages
+  static constexpr int O_COL = 128;              // TMEM: S (and P) of block j at 64 (j & 1), O
+  static constexpr int THREADS = 224;
 };
 
 template <int DT>
 struct WattnFwdSmem {
   using Cfg = WattnFwdCfg<DT>;
-  alignas(1024) uint8_t q[Cfg::TILE];
+  alignas(1024) uint8_t q[Cfg::Q_TILE];
   alignas(1024) uint8_t k[Cfg::NS][Cfg::TILE];
   alignas(1024) uint8_t v[Cfg::NS][Cfg::TILE];
-  uint64_t q_full, k_full[Cfg::NS], k_empty[Cfg::NS], v_full[Cfg::NS], v_empty[Cfg::NS];
-  uint64_t s_full, s_free, p_full, pv_done;
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2];
+  uint64_t s_full[2], p_full[2], pv_done[2];  // of block j at j & 1
   uint32_t tmem_base;
   int abort;
 };
@@ -103,7 +102,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
   const int h = blockIdx.x / a.tiles % a.Hq;
   const int b = blockIdx.x / a.tiles / a.Hq;
   const int q0 = tile * 128;
-  const WattnBlocks<7> blk(q0, a.Nq, a.Nk, a.left, a.right, a.sinks);
+  const WattnBlocks<6> blk(q0, a.Nq, a.Nk, a.left, a.right, a.sinks);
 
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
@@ -111,12 +110,12 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
       mbar_init(&sm.k_full[s], 1);
       mbar_init(&sm.k_empty[s], 1);
       mbar_init(&sm.v_full[s], 1);
-      mbar_init(&sm.v_empty[s], 1);
+      mbar_init(&sm.pv_done[s], 1);
     }
-    mbar_init(&sm.s_full, 1);
-    mbar_init(&sm.s_free, 4);
-    mbar_init(&sm.p_full, 4);
-    mbar_init(&sm.pv_done, 1);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sm.s_full[s], 1);
+      mbar_init(&sm.p_full[s], 4);
+    }
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -132,65 +131,60 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
   if (warp == 0) {
     if (lane == 0) {
       const int hk = h / a.group;
-      auto load = [&](const CUtensorMap* m, uint8_t* dst, uint64_t* bar, int head, int row, int rows) {
+      auto load = [&](const CUtensorMap* m, uint8_t* dst, uint64_t* bar, int head, int row, int rows, int sub) {
         mbar_expect_tx(bar, SUB * rows * 128);
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) tma_load_4d(dst + s * 128 * 128, m, bar, s * 64, head, row, b);
+        for (int s = 0; s < SUB; ++s) tma_load_4d(dst + s * sub, m, bar, s * 64, head, row, b);
       };
-      load(&map_q, sm.q, &sm.q_full, h, q0, 128);
+      load(&map_q, sm.q, &sm.q_full, h, q0, 128, 128 * 128);
       for (int j = 0; j < blk.n; ++j) {
         const int s = j % NS;
         const uint32_t ph = ((j / NS) & 1) ^ 1;
         const bool nar = blk.narrow(j);
-        const int rows = nar ? 32 : 128;
+        const int rows = nar ? 32 : Cfg::BK;
         if (!mbar_wait(&sm.k_empty[s], ph, abort, 501)) break;
-        load(nar ? &map_k32 : &map_k, sm.k[s], &sm.k_full[s], hk, blk.key(j), rows);
-        if (!mbar_wait(&sm.v_empty[s], ph, abort, 502)) break;
-        load(nar ? &map_v32 : &map_v, sm.v[s], &sm.v_full[s], hk, blk.key(j), rows);
+        load(nar ? &map_k32 : &map_k, sm.k[s], &sm.k_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
+        if (!mbar_wait(&sm.pv_done[s], ph, abort, 502)) break;  // P v of the block before in this stage
+        load(nar ? &map_v32 : &map_v, sm.v[s], &sm.v_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc_pv = make_idesc_f16(128, DT, E::kFmt, false, true);
+      // S of block j; its buffer held P of block j - 2
       const int ksteps = (a.D + 15) >> 4;
       const uint32_t qa = smem_u32(sm.q);
-      auto issue_s = [&](int j) {
-        const int s = j % NS;
-        if (!mbar_wait(&sm.k_full[s], (j / NS) & 1, abort, 503)) return false;
+      bool ok = mbar_wait(&sm.q_full, 0, abort, 504);
+      for (int j = 0; ok && j < blk.n; ++j) {
+        const int s = j & 1;
+        if (!mbar_wait(&sm.k_full[s], (j >> 1) & 1, abort, 503)) break;
+        if (!mbar_wait(&sm.pv_done[s], ((j >> 1) & 1) ^ 1, abort, 505)) break;
         tc_fence_after();
-        const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : 128, E::kFmt, false, false);
+        const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : Cfg::BK, E::kFmt, false, false);
         const uint32_t ka = smem_u32(sm.k[s]);
 #pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk) {
-          const uint32_t off = (kk / 4) * 128 * 128 + (kk % 4) * 32;
+        for (int kk = 0; kk < DT / 16; ++kk)
           if (kk < ksteps)
-            mma_ss(tbase + Cfg::S_COL, make_smem_desc(qa + off, 16, 1024, kSw128),
-                   make_smem_desc(ka + off, 16, 1024, kSw128), idesc, kk > 0);
-        }
-        mma_commit(&sm.s_full);
-        mma_commit(&sm.k_empty[s]);
-        return true;
-      };
-      bool ok = mbar_wait(&sm.q_full, 0, abort, 504) && issue_s(0);
-      for (int j = 0; ok && j < blk.n; ++j) {
-        if (Cfg::AHEAD && j + 1 < blk.n) {
-          if (!mbar_wait(&sm.s_free, j & 1, abort, 505)) break;
-          if (!issue_s(j + 1)) break;
-        }
-        const int s = j % NS;
-        if (!mbar_wait(&sm.v_full[s], (j / NS) & 1, abort, 506)) break;
-        if (!mbar_wait(&sm.p_full, j & 1, abort, 507)) break;
+            mma_ss(tbase + s * 64, make_smem_desc(qa + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
+                   make_smem_desc(ka + (kk / 4) * Cfg::BK * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
+        mma_commit(&sm.s_full[s]);
+      }
+    }
+  } else if (warp == 6) {
+    if (lane == 0) {
+      const uint32_t idesc_pv = make_idesc_f16(128, DT, E::kFmt, false, true);
+      for (int j = 0; j < blk.n; ++j) {
+        const int s = j & 1;
+        if (!mbar_wait(&sm.v_full[s], (j >> 1) & 1, abort, 506)) break;
+        if (!mbar_wait(&sm.p_full[s], (j >> 1) & 1, abort, 507)) break;
         tc_fence_after();
         const uint32_t va = smem_u32(sm.v[s]);
-        const int steps = blk.narrow(j) ? 2 : 8;
+        const int steps = blk.narrow(j) ? 2 : 4;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
+        for (int kk = 0; kk < 4; ++kk)
           if (kk < steps)
-            mma_ts(tbase + Cfg::O_COL, tbase + Cfg::P_COL + kk * 8, make_smem_desc(va + kk * 2048, 16384, 1024, kSw128),
-                   idesc_pv, j > 0 || kk > 0);
-        mma_commit(&sm.pv_done);
-        mma_commit(&sm.v_empty[s]);
-        if (!Cfg::AHEAD && j + 1 < blk.n && !issue_s(j + 1)) break;
+            mma_ts(tbase + Cfg::O_COL, tbase + s * 64 + kk * 8,
+                   make_smem_desc(va + kk * 2048, Cfg::BK * 128, 1024, kSw128), idesc_pv, j > 0 || kk > 0);
+        mma_commit(&sm.pv_done[s]);
       }
     }
   } else {
@@ -203,48 +197,44 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     float m = -INFINITY, l = 0.f;
     bool ok = true;
 
-    // one block of NCOL keys
-    auto work = [&](auto ncol_c, int j, int key, bool edge, const uint32_t* kept) {
+    // One block of NCOL keys; EDGE: some of them may not be seen.
+    auto work = [&](auto ncol_c, auto edge_c, int j, int key, const uint32_t* kept) {
       constexpr int NCOL = decltype(ncol_c)::value;
+      constexpr bool EDGE = decltype(edge_c)::value;
+      const uint32_t s_addr = lane_addr + (j & 1) * 64;
       uint32_t x[NCOL];
-      if constexpr (NCOL == 128) {
-        tmem_ld64_async(lane_addr + Cfg::S_COL, x);
-        tmem_ld64_async(lane_addr + Cfg::S_COL + 64, x + 64);
-        tmem_wait_ld64(x);
-        tmem_wait_ld64(x + 64);
-      } else {
-        tmem_ld32(lane_addr + Cfg::S_COL, x);
-      }
-      if (Cfg::AHEAD) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.s_free);
-      }
-      if (edge) {
-        const int first = blk.sink(j) ? blk.nse : lo, upto = blk.sink(j) ? blk.nse : a.sinks;
+      if constexpr (NCOL == 64)
+        tmem_ld64(s_addr, x);
+      else
+        tmem_ld32(s_addr, x);
+      if constexpr (EDGE) {
+        const bool snk = blk.sink(j);
+        const int first = snk ? blk.nse : lo, upto = snk ? blk.nse : a.sinks, end = snk ? min(hi, blk.nse) : hi;
 #pragma unroll
         for (int w = 0; w < NCOL / 32; ++w) {
           const int k0 = key + w * 32;
-          uint32_t see = bits_below(hi - k0) & (~bits_below(first - k0) | bits_below(upto - k0));
-          if (blk.sink(j)) see &= bits_below(blk.nse - k0);
+          uint32_t see = bits_below(end - k0) & (~bits_below(first - k0) | bits_below(upto - k0));
           if (MASK) see &= kept[w];
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (!(see >> i & 1)) x[w * 32 + i] = 0xff800000u;  // -inf
         }
       }
-      float t[8];
+      float t[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = __uint_as_float(x[i]);
+      for (int i = 0; i < 4; ++i) t[i] = __uint_as_float(x[i]);
 #pragma unroll
-      for (int i = 8; i < NCOL; ++i) t[i & 7] = fmaxf(t[i & 7], __uint_as_float(x[i]));
-      const float mx = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+      for (int i = 4; i < NCOL; i += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          t[e] = fmaxf(fmaxf(t[e], __uint_as_float(x[i + e])), i + 4 + e < NCOL ? __uint_as_float(x[i + 4 + e]) : t[e]);
+      const float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
       const bool need = m == -INFINITY ? mx > -INFINITY : mx > m + grow;
       if (__any_sync(0xffffffffu, need)) {
         const float mn = need ? mx : m;
         if (j > 0) {
           // O is stable once P v of the block before is done
-          if (!mbar_wait(&sm.pv_done, (j - 1) & 1, abort, 508)) return false;
+          if (!mbar_wait(&sm.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort, 508)) return false;
           tc_fence_after();
           const float f = need ? ex2_approx((m - mn) * c) : 1.0f;
           l *= f;
@@ -258,21 +248,16 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
           }
         }
         m = mn;
-      } else if (Cfg::AHEAD && j > 0) {
-        // P of the block before has been read
-        if (!mbar_wait(&sm.pv_done, (j - 1) & 1, abort, 509)) return false;
-        tc_fence_after();
       }
       const float mc = m == -INFINITY ? 0.f : m * c;
-      const unsigned long long c2 = f2_pack(c, c), d2 = f2_pack(-mc, -mc);
-      unsigned long long sum[2] = {0ull, 0ull};
+      const f2 c2 = f2_both(c), d2 = f2_both(-mc);
+      f2 sum[2] = {0ull, 0ull};
 #pragma unroll
       for (int c0 = 0; c0 < NCOL; c0 += 32) {
         uint32_t pk[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const unsigned long long e =
-              f2_fma(f2_pack(__uint_as_float(x[c0 + 2 * i]), __uint_as_float(x[c0 + 2 * i + 1])), c2, d2);
+          const f2 e = f2_fma(f2_pack(__uint_as_float(x[c0 + 2 * i]), __uint_as_float(x[c0 + 2 * i + 1])), c2, d2);
           float e0, e1;
           f2_unpack(e, e0, e1);
           e0 = ex2_approx(e0);
@@ -280,7 +265,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
           sum[i & 1] = f2_add(sum[i & 1], f2_pack(e0, e1));
           pk[i] = E::pack2(e0, e1);
         }
-        tmem_st16(lane_addr + Cfg::P_COL + c0 / 2, pk);
+        tmem_st16(s_addr + c0 / 2, pk);
       }
       float s0, s1;
       f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
@@ -292,52 +277,53 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     for (int j = 0; j < blk.n; ++j) {
       const int key = blk.key(j);
       const bool nar = blk.narrow(j);
-      uint32_t kept[4];
+      uint32_t kept[2];
       bool whole = true;
       if constexpr (MASK) {
         const uint8_t* mk = a.mask + static_cast<int64_t>(b) * a.Nk;
-        uint8_t byte[4];
+        uint8_t byte[2];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < 2; ++w) {
           const int k = key + w * 32 + lane;
           byte[w] = k < a.Nk ? mk[k] : 0;
         }
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          kept[w] = __ballot_sync(0xffffffffu, byte[w] != 0);
-          whole = whole && kept[w] == 0xffffffffu;
-        }
+        kept[0] = __ballot_sync(0xffffffffu, byte[0] != 0);
+        kept[1] = __ballot_sync(0xffffffffu, byte[1] != 0);
+        whole = (kept[0] & kept[1]) == 0xffffffffu;
       }
-      if (!mbar_wait(&sm.s_full, j & 1, abort, 510)) { ok = false; break; }
+      if (!mbar_wait(&sm.s_full[j & 1], (j >> 1) & 1, abort, 510)) { ok = false; break; }
+      if (warp == 2 && lane == 0) mbar_arrive(&sm.k_empty[j & 1]);  // q k^T of the block is done
       tc_fence_after();
-      // whole tile inside every row's window: the first row's end and the last row's start
-      const bool inside = key + 128 <= min(blk.p0 + a.right + 1, a.Nk) && !blk.sink(j) &&
-                          (key >= blk.p0 + blk.rows - 1 - a.left || key + 128 <= a.sinks);
-      const bool edge = !inside || !whole;
-      const bool done = nar ? work(std::integral_constant<int, 32>(), j, key, true, kept)
-                            : work(std::integral_constant<int, 128>(), j, key, edge, kept);
+      // every row sees the whole block: up to the first row's end, from the last row's start
+      const bool inside = key + Cfg::BK <= min(blk.p0 + a.right + 1, a.Nk) && !blk.sink(j) &&
+                          (key >= blk.p0 + blk.rows - 1 - a.left || key + Cfg::BK <= a.sinks);
+      using std::integral_constant;
+      const bool done =
+          nar ? work(integral_constant<int, 32>(), integral_constant<bool, true>(), j, key, kept)
+          : inside && whole ? work(integral_constant<int, 64>(), integral_constant<bool, false>(), j, key, kept)
+                            : work(integral_constant<int, 64>(), integral_constant<bool, true>(), j, key, kept);
       if (!done) { ok = false; break; }
       if constexpr (MASK) {
         if (!whole) {
           // masked keys' rows of V: zero (the swizzle moves 16-byte chunks within a row only)
           if (!mbar_wait(&sm.v_full[j % NS], (j / NS) & 1, abort, 511)) { ok = false; break; }
-          const uint32_t word = wq == 0 ? kept[0] : wq == 1 ? kept[1] : wq == 2 ? kept[2] : kept[3];
-          if (!(word >> lane & 1) && (!nar || row < 32)) {
+          const uint32_t word = wq & 1 ? kept[1] : kept[0];
+          if (row < (nar ? 32 : 64) && !(word >> lane & 1)) {
 #pragma unroll
             for (int s = 0; s < SUB; ++s)
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                reinterpret_cast<uint4*>(sm.v[j % NS] + s * 128 * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sm.v[j % NS] + s * Cfg::BK * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full);
+      if (lane == 0) mbar_arrive(&sm.p_full[j & 1]);
     }
     // ---------------- O / l -> out, lse ----------------
-    if (ok && mbar_wait(&sm.pv_done, (blk.n - 1) & 1, abort, 512)) {
+    if (ok && mbar_wait(&sm.pv_done[(blk.n - 1) & 1], ((blk.n - 1) >> 1) & 1, abort, 512)) {
       tc_fence_after();
       const int i = q0 + row;
       const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -404,8 +390,8 @@ template <typename T, int DT, bool MASK>
 int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float* lse, cudaStream_t st) {
   CUtensorMap mq, mk, mv, mk32, mv32;
   if (!wattn_map(&mq, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 128) ||
-      !wattn_map(&mk, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 128) ||
-      !wattn_map(&mv, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 128) ||
+      !wattn_map(&mk, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 64) ||
+      !wattn_map(&mv, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64) ||
       !wattn_map(&mk32, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 32) ||
       !wattn_map(&mv32, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 32))
     return TOPS_ERR_TMAP;

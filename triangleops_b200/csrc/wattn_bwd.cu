@@ -4,13 +4,15 @@
 //   dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,  dV = P^T dO.
 // Two kernels of one shape: 128 rows stay (two operand tiles A1, A2), tiles of 64 rows stream by
 // (B1, B2). Per streamed tile, T1 = A1 B1^T and T2 = A2 B2^T (fp32, TMEM); two softmax warpgroups,
-// taking tiles in turn, make P and dS from them and put them back to TMEM rounded to the IO dtype
-// (a product's operands have one type); then
+// each with half of the tile's columns, make P and dS from them and put them back to TMEM rounded
+// to the IO dtype (a product's operands have one type); then
 //   KV: rows are keys (A = k, v; B = q, dO):    dV += P B2,  dK += dS B1
 //   Q : rows are queries (A = q, dO; B = k, v): dQ += dS B1
 // accumulate in TMEM. T1 and T2 have two buffers, so the MMAs of one tile run under the softmax of
-// the other. S and dP are computed in both kernels (7 products for the 5 of one that adds dQ up in
-// memory by atomics): nothing is added in an order that changes, and dS is not stored.
+// the other, and each product has a warp of its own to issue it: a thread takes some 90 cycles to
+// issue an MMA, and one thread for all 24 of a tile was what bound the kernel (3.5 k cycles a tile).
+// S and dP are computed in both kernels (7 products for the 5 of one that adds dQ up in memory by
+// atomics): nothing is added in an order that changes, and dS is not stored.
 //
 // KV walks the query heads of its key head one after the other, so the sum over a shared head's
 // queries stays in TMEM. A block of sink keys is seen by every later query: its walk is cut into
@@ -44,7 +46,7 @@ struct WattnBwdCfg {
   static constexpr int STR = SUB * 64 * 128;   // bytes of a streamed tile
   static constexpr int NST = 4;                // stages of streamed tiles
   static constexpr int ACC = 256;              // TMEM: T1, T2 of buffer s at 128 s and 128 s + 64
-  static constexpr int THREADS = 320;
+  static constexpr int THREADS = 416;
 };
 
 template <int DT>
@@ -55,7 +57,8 @@ struct WattnBwdSmem {
   alignas(1024) uint8_t b1[Cfg::NST][Cfg::STR];
   alignas(1024) uint8_t b2[Cfg::NST][Cfg::STR];
   alignas(16) float st[Cfg::NST][2][64];  // KV: lse2 and delta of the streamed queries
-  uint64_t res_full, full[Cfg::NST], empty[Cfg::NST], t_full[2], ds_full[2], acc_done;
+  uint64_t res_full, full[Cfg::NST], empty[Cfg::NST];
+  uint64_t t_full[2], p_full[2], ds_full[2], p_free[2], ds_free[2], acc_done;  // of tile it at it & 1
   uint32_t tmem_base;
   int abort;
 };
@@ -127,13 +130,16 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
     mbar_init(&sm.res_full, 1);
     for (int s = 0; s < NST; ++s) {
       mbar_init(&sm.full[s], 1);
-      mbar_init(&sm.empty[s], 1);
+      mbar_init(&sm.empty[s], KV ? 2 : 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&sm.t_full[s], 1);
-      mbar_init(&sm.ds_full[s], 4);
+      mbar_init(&sm.t_full[s], 2);
+      mbar_init(&sm.p_full[s], 8);
+      mbar_init(&sm.ds_full[s], 8);
+      mbar_init(&sm.p_free[s], 1);
+      mbar_init(&sm.ds_free[s], 1);
     }
-    mbar_init(&sm.acc_done, 1);
+    mbar_init(&sm.acc_done, KV ? 2 : 1);
     sm.abort = 0;
     fence_mbar_init();
   }
@@ -169,60 +175,52 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
         }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp <= 2) {
+    // T1 (warp 1) and T2 (warp 2); a buffer is free once the product that read P (KV: T1's) or dS
+    // out of it is done. (Q keeps no P: T1's goes with dS.)
     if (lane == 0 && walk.total > 0) {
-      const uint32_t idesc_t = make_idesc_f16(128, 64, E::kFmt, false, false);
-      const uint32_t idesc_acc = make_idesc_f16(128, DT, E::kFmt, false, true);
+      const uint32_t idesc = make_idesc_f16(128, 64, E::kFmt, false, false);
       const int ksteps = (a.D + 15) >> 4;
-      const uint32_t a1 = smem_u32(sm.a1), a2 = smem_u32(sm.a2);
-      auto issue_t = [&](int it) {
-        const int r = it % NST;
-        if (!mbar_wait(&sm.full[r], (it / NST) & 1, abort, 522)) return false;
-        tc_fence_after();
-        const uint32_t b1 = smem_u32(sm.b1[r]), b2 = smem_u32(sm.b2[r]);
-        const uint32_t t1 = tbase + (it & 1) * 128, t2 = t1 + 64;
-#pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk) {
-          const uint32_t oa = (kk / 4) * 128 * 128 + (kk % 4) * 32, ob = (kk / 4) * 64 * 128 + (kk % 4) * 32;
-          if (kk < ksteps)
-            mma_ss(t1, make_smem_desc(a1 + oa, 16, 1024, kSw128), make_smem_desc(b1 + ob, 16, 1024, kSw128), idesc_t,
-                   kk > 0);
-        }
-#pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk) {
-          const uint32_t oa = (kk / 4) * 128 * 128 + (kk % 4) * 32, ob = (kk / 4) * 64 * 128 + (kk % 4) * 32;
-          if (kk < ksteps)
-            mma_ss(t2, make_smem_desc(a2 + oa, 16, 1024, kSw128), make_smem_desc(b2 + ob, 16, 1024, kSw128), idesc_t,
-                   kk > 0);
-        }
-        mma_commit(&sm.t_full[it & 1]);
-        return true;
-      };
-      bool ok = mbar_wait(&sm.res_full, 0, abort, 523) && issue_t(0);
+      const uint32_t ra = smem_u32(warp == 1 ? sm.a1 : sm.a2);
+      uint64_t* const free = KV && warp == 1 ? sm.p_free : sm.ds_free;
+      bool ok = mbar_wait(&sm.res_full, 0, abort, 523);
       for (int it = 0; ok && it < walk.total; ++it) {
-        // T of the next tile: its buffer's P and dS were read by products issued before it
-        if (it + 1 < walk.total && !issue_t(it + 1)) break;
-        if (!mbar_wait(&sm.ds_full[it & 1], (it >> 1) & 1, abort, 524)) break;
+        const int r = it % NST, s = it & 1;
+        if (!mbar_wait(&sm.full[r], (it / NST) & 1, abort, 522)) break;
+        if (!mbar_wait(&free[s], ((it >> 1) & 1) ^ 1, abort, 524)) break;
         tc_fence_after();
-        const int r = it % NST;
-        const uint32_t t1 = tbase + (it & 1) * 128, t2 = t1 + 64;
-        const uint32_t b1 = smem_u32(sm.b1[r]), b2 = smem_u32(sm.b2[r]);
-        if constexpr (KV) {
+        const uint32_t rb = smem_u32(warp == 1 ? sm.b1[r] : sm.b2[r]), t = tbase + s * 128 + (warp - 1) * 64;
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ts(tbase + Cfg::ACC, t1 + kk * 8, make_smem_desc(b2 + kk * 2048, 8192, 1024, kSw128), idesc_acc,
-                   it > 0 || kk > 0);
-        }
+        for (int kk = 0; kk < DT / 16; ++kk)
+          if (kk < ksteps)
+            mma_ss(t, make_smem_desc(ra + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
+                   make_smem_desc(rb + (kk / 4) * 64 * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
+        mma_commit(&sm.t_full[s]);
+      }
+    }
+  } else if (warp <= 4) {
+    // KV: dV += P B2 (warp 3), dK += dS B1 (warp 4); Q: dQ += dS B1 (warp 4)
+    if (lane == 0 && (KV || warp == 4)) {
+      const uint32_t idesc = make_idesc_f16(128, DT, E::kFmt, false, true);
+      const bool of_p = warp == 3;
+      const uint32_t acc = tbase + Cfg::ACC + (KV && !of_p ? DT : 0);
+      for (int it = 0; it < walk.total; ++it) {
+        const int r = it % NST, s = it & 1;
+        if (!mbar_wait(of_p ? &sm.p_full[s] : &sm.ds_full[s], (it >> 1) & 1, abort, 528)) break;
+        tc_fence_after();
+        const uint32_t t = tbase + s * 128 + (of_p ? 0 : 64), rb = smem_u32(of_p ? sm.b2[r] : sm.b1[r]);
+        // a warpgroup leaves its 32 columns, packed to 16, where they were: at 0 and 32
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk)
-          mma_ts(tbase + Cfg::ACC + (KV ? DT : 0), t2 + kk * 8, make_smem_desc(b1 + kk * 2048, 8192, 1024, kSw128),
-                 idesc_acc, it > 0 || kk > 0);
+          mma_ts(acc, t + (kk >> 1) * 32 + (kk & 1) * 8, make_smem_desc(rb + kk * 2048, 64 * 128, 1024, kSw128), idesc,
+                 it > 0 || kk > 0);
+        mma_commit(of_p ? &sm.p_free[s] : &sm.ds_free[s]);
         mma_commit(&sm.empty[r]);
         if (it + 1 == walk.total) mma_commit(&sm.acc_done);
       }
     }
   } else {
-    const int g = (warp - 2) >> 2;  // warpgroup: tiles g, g + 2, ...
+    const int g = (warp - 5) >> 2;  // warpgroup: columns 32 g .. of every tile
     const int wq = warp & 3;
     const int row = wq * 32 + lane;
     const uint32_t lane_addr = tbase + (static_cast<uint32_t>(wq * 32) << 16);
@@ -247,108 +245,110 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
       lse2 = a.lse2[q];
       delta = a.delta[q];
     }
-    const unsigned long long c2 = f2_pack(a.c, a.c);
+    const f2 c2 = f2_both(a.c);
     bool ok = true;
-    for (int it = g; it < walk.total; it += 2) {
-      const int r = it % NST, r0 = walk.row(it);
-      uint32_t kept[2] = {0xffffffffu, 0xffffffffu};
+    for (int it = 0; it < walk.total; ++it) {
+      const int r = it % NST, s = it & 1, r0 = walk.row(it) + 32 * g;  // this warpgroup's first streamed row
+      uint32_t kept = 0xffffffffu;
       bool whole = keep;
       if (!KV && a.mask) {
-        const uint8_t* mk = a.mask + static_cast<int64_t>(walk.b) * a.Nk;
-        uint8_t byte[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int k = r0 + w * 32 + lane;
-          byte[w] = k < a.Nk ? mk[k] : 0;
-        }
-        kept[0] = __ballot_sync(0xffffffffu, byte[0] != 0);
-        kept[1] = __ballot_sync(0xffffffffu, byte[1] != 0);
-        whole = (kept[0] & kept[1]) == 0xffffffffu;
+        const int k = r0 + lane;
+        const uint8_t byte = k < a.Nk ? a.mask[static_cast<int64_t>(walk.b) * a.Nk + k] : 0;
+        kept = __ballot_sync(0xffffffffu, byte != 0);
+        whole = kept == 0xffffffffu;
       }
       if (KV && !mbar_wait(&sm.full[r], (it / NST) & 1, abort, 525)) { ok = false; break; }
-      if (!mbar_wait(&sm.t_full[g], (it >> 1) & 1, abort, 526)) { ok = false; break; }
+      if (!mbar_wait(&sm.t_full[s], (it >> 1) & 1, abort, 526)) { ok = false; break; }
       tc_fence_after();
-      uint32_t x[64], y[64];
-      const uint32_t t1 = lane_addr + g * 128, t2 = t1 + 64;
-      tmem_ld64_async(t1, x);
-      tmem_ld64_async(t2, y);
-      tmem_wait_ld64(x);
-      tmem_wait_ld64(y);
+      uint32_t x[32], y[32];
+      const uint32_t t1 = lane_addr + s * 128 + 32 * g, t2 = t1 + 64;
+      tmem_ld32(t1, x);
       bool inside;
       if constexpr (KV) {
         const int p0 = r0 + off;
-        inside = p0 >= walk.row0 + 127 - a.right && p0 + 63 <= walk.row0 + a.left;
+        inside = p0 >= walk.row0 + 127 - a.right && p0 + 31 <= walk.row0 + a.left;
       } else {
         const int p0 = walk.row0 + off;
-        inside = r0 + 64 <= min(p0 + a.right + 1, a.Nk) && !walk.blk.sink(it) &&
-                 (r0 >= p0 + walk.blk.rows - 1 - a.left || r0 + 64 <= a.sinks);
+        inside = r0 + 32 <= min(p0 + a.right + 1, a.Nk) && !walk.blk.sink(it) &&
+                 (r0 >= p0 + walk.blk.rows - 1 - a.left || r0 + 32 <= a.sinks);
       }
-      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      uint32_t see = 0xffffffffu;
       const bool edge = __any_sync(0xffffffffu, !inside || !whole);
       if (edge) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if constexpr (KV) {
-            const int b0 = r0 + off + w * 32;
-            see[w] = keep ? bits_below(hi - b0) & ~bits_below(lo - b0) : 0u;
-          } else {
-            const int b0 = r0 + w * 32;
-            const bool snk = walk.blk.sink(it);
-            const int f = snk ? walk.blk.nse : lo, u = snk ? walk.blk.nse : upto;
-            see[w] = bits_below(hi - b0) & (~bits_below(f - b0) | bits_below(u - b0)) & kept[w];
-            if (snk) see[w] &= bits_below(walk.blk.nse - b0);
-          }
+        if constexpr (KV) {
+          const int b0 = r0 + off;
+          see = keep ? bits_below(hi - b0) & ~bits_below(lo - b0) : 0u;
+        } else {
+          const bool snk = walk.blk.sink(it);
+          const int f = snk ? walk.blk.nse : lo, u = snk ? walk.blk.nse : upto, e = snk ? min(hi, walk.blk.nse) : hi;
+          see = bits_below(e - r0) & (~bits_below(f - r0) | bits_below(u - r0)) & kept;
         }
       }
-      const float* s_lse = sm.st[r][0];
-      const float* s_del = sm.st[r][1];
+      const float* s_lse = sm.st[r][0] + 32 * g;
+      const float* s_del = sm.st[r][1] + 32 * g;
+      uint32_t pk[16];
 #pragma unroll
-      for (int c0 = 0; c0 < 64; c0 += 32) {
-        uint32_t pk[16], dk[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int e = c0 + 2 * i;
-          unsigned long long nl, nd;
-          if constexpr (KV) {
-            nl = f2_pack(-s_lse[e], -s_lse[e + 1]);
-            nd = f2_pack(-s_del[e], -s_del[e + 1]);
-          } else {
-            nl = f2_pack(-lse2, -lse2);
-            nd = f2_pack(-delta, -delta);
-          }
-          float p0, p1, d0, d1;
-          f2_unpack(f2_fma(f2_pack(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), c2, nl), p0, p1);
-          p0 = ex2_approx(p0);
-          p1 = ex2_approx(p1);
-          f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(y[e]), __uint_as_float(y[e + 1])), nd), f2_pack(p0, p1)), d0,
-                    d1);
-          if (edge) {
-            const uint32_t w = see[c0 / 32] >> (2 * i);
-            if (!(w & 1)) p0 = d0 = 0.f;
-            if (!(w & 2)) p1 = d1 = 0.f;
-          }
-          if constexpr (KV) pk[i] = E::pack2(p0, p1);
-          dk[i] = E::pack2(d0, d1);
+      for (int i = 0; i < 16; ++i) {
+        f2 nl;
+        if constexpr (KV)
+          nl = f2_pack(-s_lse[2 * i], -s_lse[2 * i + 1]);
+        else
+          nl = f2_both(-lse2);
+        float p0, p1;
+        f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, nl), p0, p1);
+        p0 = ex2_approx(p0);
+        p1 = ex2_approx(p1);
+        if (edge) {
+          const uint32_t w = see >> (2 * i);
+          if (!(w & 1)) p0 = 0.f;
+          if (!(w & 2)) p1 = 0.f;
         }
-        if constexpr (KV) tmem_st16(t1 + c0 / 2, pk);
-        tmem_st16(t2 + c0 / 2, dk);
+        x[2 * i] = __float_as_uint(p0);
+        x[2 * i + 1] = __float_as_uint(p1);
+        if constexpr (KV) pk[i] = E::pack2(p0, p1);
       }
-      if (!KV && a.mask && !whole) {
+      if constexpr (KV) {
+        tmem_st16(t1, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.p_full[s]);
+      }
+      tmem_ld32(t2, y);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        f2 nd;
+        if constexpr (KV)
+          nd = f2_pack(-s_del[2 * i], -s_del[2 * i + 1]);
+        else
+          nd = f2_both(-delta);
+        float d0, d1;
+        f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), nd),
+                         f2_pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))),
+                  d0, d1);
+        if (edge) {  // (what an unseen pair's product holds may be NaN)
+          const uint32_t w = see >> (2 * i);
+          if (!(w & 1)) d0 = 0.f;
+          if (!(w & 2)) d1 = 0.f;
+        }
+        pk[i] = E::pack2(d0, d1);
+      }
+      tmem_st16(t2, pk);
+      if (!KV && a.mask && !whole && wq == 0) {
         // T1 of this tile is done: its masked keys' rows may be zeroed for dS k
-        const uint32_t word = row < 32 ? kept[0] : kept[1];
-        if (row < 64 && !(word >> lane & 1)) {
+        if (!(kept >> lane & 1)) {
 #pragma unroll
-          for (int s = 0; s < SUB; ++s)
+          for (int u = 0; u < SUB; ++u)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              reinterpret_cast<uint4*>(sm.b1[r] + s * 64 * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
+              reinterpret_cast<uint4*>(sm.b1[r] + u * 64 * 128 + (32 * g + lane) * 128)[i] = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.ds_full[g]);
+      if (lane == 0) mbar_arrive(&sm.ds_full[s]);
     }
     // ---------------- epilogue ----------------
     // KV: warpgroup 0 writes dV, 1 dK; Q: each half of dQ's channels
