@@ -433,6 +433,11 @@ __device__ __forceinline__ uint32_t ex2_poly_f16x2(uint32_t x) {
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(p), "r"(scale));
   return y;
 }
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 __device__ __forceinline__ float tanh_approx(float x) {
   float y;
   asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
