@@ -217,6 +217,32 @@ def test_autograd(device):
         assert torch.equal(a, b)
 
 
+@gpu
+def test_first_use_in_a_new_thread(device):
+    """A thread that has made no CUDA call yet (as autograd's are)."""
+    import threading
+
+    q, k, v, d = _inputs(device, BF, 1, 200, 200, 2, 1, 64)
+    want, lse = window_attn.forward(q, k, v, window=64, sinks=1)
+    torch.cuda.synchronize()
+    got = []
+
+    def work(f):
+        try:
+            got.append(f())
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    for f in (lambda: window_attn.forward(q, k, v, window=64, sinks=1)[0],
+              lambda: window_attn.backward(d, q, k, v, want, lse, window=64, sinks=1)[2]):
+        t = threading.Thread(target=work, args=(f,))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want)
+    assert torch.equal(got[1], window_attn.backward(d, q, k, v, want, lse, window=64, sinks=1)[2])
+
+
 def _decode_ref(q, k, v, lengths, window, sinks):
     out, err = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64)
     for b, n in enumerate(lengths.tolist()):

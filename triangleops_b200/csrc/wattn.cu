@@ -21,6 +21,7 @@
 //
 // Masked keys: their score is replaced by -inf, and their rows of the V tile are zeroed in shared
 // memory before P v, so that a NaN there does not pass through 0 * NaN.
+#include <atomic>
 #include "sm100.cuh"
 #include "wattn.h"
 
@@ -358,6 +359,18 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+// A thread that has not used its device yet (autograd has threads of its own) has no current context,
+// without which a tensor map cannot be encoded; the first runtime call that needs one makes it.
+inline void bind_context() {
+  static thread_local uint64_t bound = 0;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (bound & bit) return;
+  cudaFree(nullptr);
+  bound |= bit;
+}
+
 // (B, N, H, D) with channel rows of D elements: boxes of 64 channels x `rows` tokens of one head,
 // 128B swizzle. A place of size 1 gets a stride of one row whatever the tensor says.
 inline bool wattn_map(CUtensorMap* m, int dtype, const void* p, const int64_t* st, int64_t B, int64_t N, int64_t H,
@@ -386,14 +399,29 @@ inline bool wattn_tensor(int dtype, const WattnArgs& a) {
          wattn_fits(a.v, a.vs, a.B, a.Nk, a.Hkv);
 }
 
+// The kernel's shared memory limit, raised once a device (the call costs as much as a launch).
+template <typename K>
+inline void set_smem_once(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  set_smem(kernel, bytes);
+  done.fetch_or(bit, std::memory_order_relaxed);
+}
+
 template <typename T, int DT, bool MASK>
 int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float* lse, cudaStream_t st) {
+  bind_context();
   CUtensorMap mq, mk, mv, mk32, mv32;
   if (!wattn_map(&mq, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 128) ||
       !wattn_map(&mk, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 64) ||
-      !wattn_map(&mv, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64) ||
-      !wattn_map(&mk32, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 32) ||
-      !wattn_map(&mv32, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 32))
+      !wattn_map(&mv, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64))
+    return TOPS_ERR_TMAP;
+  if (a.sinks == 0)  // no block of left-behind sinks
+    mk32 = mk, mv32 = mv;
+  else if (!wattn_map(&mk32, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 32) ||
+           !wattn_map(&mv32, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 32))
     return TOPS_ERR_TMAP;
   WattnFwdArgs f;
   f.Nq = a.Nq, f.Nk = a.Nk, f.Hq = a.Hq, f.group = a.Hq / a.Hkv, f.D = a.D;
@@ -403,7 +431,8 @@ int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float* lse, c
   if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   const size_t smem = sizeof(WattnFwdSmem<DT>) + 1024;
   auto kern = wattn_forward_kernel<T, DT, MASK>;
-  set_smem(kern, smem);
+  static std::atomic<uint64_t> done{0};
+  set_smem_once(kern, smem, done);
   kern<<<static_cast<unsigned>(grid), WattnFwdCfg<DT>::THREADS, smem, st>>>(mq, mk, mv, mk32, mv32, f);
   return launch_status();
 }

@@ -15,8 +15,10 @@
 // atomics): nothing is added in an order that changes, and dS is not stored.
 //
 // KV walks the query heads of its key head one after the other, so the sum over a shared head's
-// queries stays in TMEM. A block of sink keys is seen by every later query: its walk is cut into
-// `nch` parts of about the length of the other blocks', whose fp32 sums a last kernel adds in order.
+// queries stays in TMEM. The queries that see a tile's sinks only as sinks, all those past its window,
+// are the work of further, shorter blocks behind the tiles' own (a quarter of their length, so that
+// they fill the SMs that the last round of tiles leaves idle); their fp32 sums, and the tile's
+// own for these rows, are added in order by a last kernel.
 //
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
@@ -30,13 +32,15 @@ struct WattnBwdArgs {
   int Nq, Nk, Hq, Hkv, group, D;
   int left, right, sinks;
   int tiles;             // Q: query tiles; KV: key tiles
-  int nsb, nch;          // KV: tiles with sinks, parts of their walk
+  int own;               // KV: blocks of the tiles themselves; behind them, for the sinks' late queries,
+  int nsb, nx, per;      // of nsb tiles and each query head, nx blocks of `per` streamed tiles
+  int keep;              // rows of a part
   int nqp;               // row length of lse2 and delta
   const uint8_t* mask;
   float c, scale;
   const float *lse2, *delta;  // [B][Hq][nqp]
   void *d1, *d2;              // KV: dv, dk; Q: dq
-  float* part;                // [B][Hkv][nsb][nch][2][128][DT]
+  float* part;                // [B][Hkv][nsb][1 + group nx][2][keep][DT]
 };
 
 template <int DT>
@@ -66,29 +70,41 @@ struct WattnBwdSmem {
 // The walk of one block: which tiles stream by.
 template <bool KV>
 struct WattnWalk {
-  int b, row0, total;     // first resident row (key or query), streamed tiles
-  int head;               // KV: first query head of the group; Q: the query head
-  int hk, first, qlo, nqb, kb, chunk;
-  WattnBlocks<6> blk;     // Q: the key tiles
+  int b, hk, row0, total;  // first resident row (key or query), streamed tiles
+  int head;                // KV: first query head; Q: the query head
+  int qlo, nqb;            // KV: first streamed query, streamed tiles of a head
+  int kb, slot;            // KV: the tile, and which of its parts this is (0: its own)
+  int late;                // KV: first query that sees the tile's sinks only as sinks
+  WattnBlocks<6> blk;      // Q: the key tiles
   __device__ WattnWalk(const WattnBwdArgs& a) : blk(0, 1, 1, 0, 0, 0) {
     if constexpr (KV) {
-      const int units = a.nsb * a.nch + a.tiles - a.nsb;
-      const int bh = blockIdx.x / units, u = blockIdx.x % units;
+      const int off = a.Nk - a.Nq;
+      int bh, u = blockIdx.x;
+      if (u < a.own) {
+        bh = u / a.tiles;
+        kb = u % a.tiles;
+        slot = 0;
+      } else {
+        u -= a.own;
+        slot = 1 + u % (a.nx * a.group);
+        u /= a.nx * a.group;
+        kb = u % a.nsb;
+        bh = u / a.nsb;
+      }
       b = bh / a.Hkv;
       hk = bh % a.Hkv;
-      head = hk * a.group;
-      const bool cut = u < a.nsb * a.nch;
-      kb = cut ? u / a.nch : u - a.nsb * a.nch + a.nsb;
-      chunk = cut ? u % a.nch : 0;
       row0 = kb * 128;
-      const int off = a.Nk - a.Nq, last = min(row0 + 127, a.Nk - 1);
-      qlo = max(0, row0 - a.right - off) & ~7;
-      const int qhi = row0 < a.sinks ? a.Nq : min(a.Nq, last + a.left + 1 - off);
-      nqb = (max(0, qhi - qlo) + 63) >> 6;
-      const int64_t all = static_cast<int64_t>(nqb) * a.group;
-      const int parts = cut ? a.nch : 1;
-      first = static_cast<int>(all * chunk / parts);
-      total = static_cast<int>(all * (chunk + 1) / parts) - first;
+      late = max(0, min(a.Nq, min(row0 + 127, a.Nk - 1) + a.left + 1 - off));
+      head = hk * a.group;
+      if (slot == 0) {
+        qlo = max(0, row0 - a.right - off) & ~7;
+        nqb = (max(0, late - qlo) + 63) >> 6;
+        total = nqb * a.group;
+      } else {
+        head += (slot - 1) / a.nx;
+        qlo = (late & ~7) + (slot - 1) % a.nx * a.per * 64;
+        total = nqb = min(a.per, (max(0, a.Nq - qlo) + 63) >> 6);
+      }
     } else {
       const int tile = blockIdx.x % a.tiles;
       head = blockIdx.x / a.tiles % a.Hq;
@@ -96,18 +112,17 @@ struct WattnWalk {
       hk = head / a.group;
       row0 = tile * 128;
       blk = WattnBlocks<6>(row0, a.Nq, a.Nk, a.left, a.right, a.sinks);
-      first = 0;
       total = blk.n;
-      qlo = nqb = kb = chunk = 0;
+      qlo = nqb = kb = slot = late = 0;
     }
   }
   // first row of streamed tile `it`, and its query head
   __device__ int row(int it) const {
-    if constexpr (KV) return qlo + (first + it) % nqb * 64;
+    if constexpr (KV) return qlo + it % nqb * 64;
     return blk.key(it);
   }
   __device__ int qhead(int it) const {
-    if constexpr (KV) return head + (first + it) / nqb;
+    if constexpr (KV) return head + it / nqb;
     return head;
   }
 };
@@ -116,7 +131,7 @@ template <typename T, int DT, bool KV>
 __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
     wattn_backward_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
                           const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2,
-                          const WattnBwdArgs a) {
+                          const WattnBwdArgs a) {  // maps: boxes of 64 rows
   using Cfg = WattnBwdCfg<DT>;
   using E = Elem<T>;
   constexpr int NST = Cfg::NST, SUB = Cfg::SUB;
@@ -154,9 +169,10 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
       const int res_head = KV ? walk.hk : walk.head;
       mbar_expect_tx(&sm.res_full, 2 * Cfg::RES);
 #pragma unroll
-      for (int s = 0; s < SUB; ++s) {
-        tma_load_4d(sm.a1 + s * 128 * 128, &map_a1, &sm.res_full, s * 64, res_head, walk.row0, walk.b);
-        tma_load_4d(sm.a2 + s * 128 * 128, &map_a2, &sm.res_full, s * 64, res_head, walk.row0, walk.b);
+      for (int s = 0; s < 2 * SUB; ++s) {
+        const int sub = s >> 1, half = (s & 1) * 64, at = sub * 128 * 128 + half * 128;
+        tma_load_4d(sm.a1 + at, &map_a1, &sm.res_full, sub * 64, res_head, walk.row0 + half, walk.b);
+        tma_load_4d(sm.a2 + at, &map_a2, &sm.res_full, sub * 64, res_head, walk.row0 + half, walk.b);
       }
       for (int it = 0; it < walk.total; ++it) {
         const int r = it % NST;
@@ -233,7 +249,9 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
     float lse2 = 0.f, delta = 0.f;
     if constexpr (KV) {
       lo = at - a.right;
-      hi = at < a.sinks ? a.Nk : at + a.left + 1;
+      hi = at + a.left + 1;
+      if (at < a.sinks) hi = walk.slot == 0 ? walk.late + off : a.Nk;
+      if (walk.slot > 0) lo = max(lo, walk.late + off);
       if (a.mask && at < a.Nk) keep = a.mask[static_cast<int64_t>(walk.b) * a.Nk + at] != 0;
     } else {
       const int p = at + off;
@@ -363,16 +381,15 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
       float* part = nullptr;
       T* dst;
       if constexpr (KV) {
-        if (a.nch > 1 && walk.kb < a.nsb)
-          part = a.part +
-                 ((((static_cast<int64_t>(walk.b) * a.Hkv + walk.hk) * a.nsb + walk.kb) * a.nch + walk.chunk) * 2 + g) *
-                     128 * DT +
-                 row * DT;
+        // (a row that only some warps' lanes own: they all load, and store what is theirs)
+        if (a.nx > 0 && walk.kb < a.nsb && row < min(a.keep, a.sinks - walk.row0))
+          part = a.part + ((((static_cast<int64_t>(walk.b) * a.Hkv + walk.hk) * a.nsb + walk.kb) *
+                                (1 + a.group * a.nx) + walk.slot) * 2 + g) * a.keep * DT + row * DT;
         dst = static_cast<T*>(g == 0 ? a.d1 : a.d2) + ((static_cast<int64_t>(walk.b) * a.Nk + at) * a.Hkv + walk.hk) * a.D;
       } else {
         dst = static_cast<T*>(a.d1) + ((static_cast<int64_t>(walk.b) * a.Nq + at) * a.Hq + walk.head) * a.D + col0;
       }
-      const bool live = at < (KV ? a.Nk : a.Nq);
+      const bool live = at < (KV ? a.Nk : a.Nq) && (!KV || walk.slot == 0);
 #pragma unroll
       for (int c0 = 0; c0 < COLS; c0 += 32) {
         uint32_t o[32];
@@ -405,7 +422,7 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
 
 // delta = sum_d dO O and lse2 = lse log2(e) per query, in rows of nqp: queries past Nq, and those
 // that see nothing, get lse2 = +inf and delta = 0. Eight threads a query, 16-byte loads.
-template <typename T>
+template <typename T, int DT>
 __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* __restrict__ dout, int64_t s0,
                                                           int64_t s1, int64_t s2, const T* __restrict__ out,
                                                           const float* __restrict__ lse, int nqp,
@@ -413,31 +430,40 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
   using E = Elem<T>;
   const int i = static_cast<int>((blockIdx.x * 256u + threadIdx.x) >> 3), part = threadIdx.x & 7;
   const int h = blockIdx.y, b = blockIdx.z;
-  float x = 0.f;
+  const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
+  float x = 0.f, v = -INFINITY;
   if (i < a.Nq) {
     const T* d = dout + b * s0 + i * s1 + h * s2;
     const T* o = out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D;
-    for (int c = part * 8; c < a.D; c += 64) {
-      const uint4 u = *reinterpret_cast<const uint4*>(d + c), w = *reinterpret_cast<const uint4*>(o + c);
-      x = fmaf(E::lo(u.x), E::lo(w.x), fmaf(E::hi(u.x), E::hi(w.x), x));
-      x = fmaf(E::lo(u.y), E::lo(w.y), fmaf(E::hi(u.y), E::hi(w.y), x));
-      x = fmaf(E::lo(u.z), E::lo(w.z), fmaf(E::hi(u.z), E::hi(w.z), x));
-      x = fmaf(E::lo(u.w), E::lo(w.w), fmaf(E::hi(u.w), E::hi(w.w), x));
+    uint4 u[DT / 64], w[DT / 64];
+#pragma unroll
+    for (int k = 0; k < DT / 64; ++k) {
+      const int c = part * 8 + 64 * k;
+      u[k] = w[k] = make_uint4(0, 0, 0, 0);
+      if (c < a.D) {
+        u[k] = *reinterpret_cast<const uint4*>(d + c);
+        w[k] = *reinterpret_cast<const uint4*>(o + c);
+      }
+    }
+    if (part == 0) v = lse[bh * a.Nq + i];
+#pragma unroll
+    for (int k = 0; k < DT / 64; ++k) {
+      const uint32_t *p = &u[k].x, *q = &w[k].x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x = fmaf(E::lo(p[e]), E::lo(q[e]), fmaf(E::hi(p[e]), E::hi(q[e]), x));
     }
   }
 #pragma unroll
   for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   if (part == 0 && i < nqp) {
-    const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
-    const float v = i < a.Nq ? lse[bh * a.Nq + i] : -INFINITY;
     lse2[bh * nqp + i] = v == -INFINITY ? INFINITY : v * kLog2e;
     delta[bh * nqp + i] = v == -INFINITY ? 0.f : x;
   }
 }
 
-// Adds the parts of the sink tiles' walks, in order. One block a (b, key head, tile, output, 8 rows).
+// Adds the parts of the sinks' rows, in order. One block: a (b, key head), tile, output, some rows.
 template <typename T, int DT>
-__global__ void __launch_bounds__(256) wattn_parts_kernel(WattnBwdArgs a) {
+__global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) {
   using E = Elem<T>;
   constexpr int PER = DT / 8;  // threads a row, 8 channels each
   constexpr int ROWS = 256 / PER;
@@ -445,10 +471,12 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(WattnBwdArgs a) {
   const int which = blockIdx.y & 1, kb = blockIdx.y >> 1;
   const int64_t bh = blockIdx.z;
   const int key = kb * 128 + row;
-  if (row >= 128 || key >= a.Nk || col >= a.D) return;
-  const float* p = a.part + ((bh * a.nsb + kb) * a.nch * 2 + which) * 128 * DT + row * DT + col;
+  if (row >= a.keep || key >= a.sinks || col >= a.D) return;
+  const int n = 1 + a.group * a.nx;
+  const float* p = a.part + ((bh * a.nsb + kb) * n * 2 + which) * a.keep * DT + row * DT + col;
   float v[8] = {};
-  for (int n = 0; n < a.nch; ++n, p += 2 * 128 * DT) {
+#pragma unroll 4
+  for (int i = 0; i < n; ++i, p += 2 * a.keep * DT) {
     const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
     v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
     v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
@@ -464,8 +492,8 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(WattnBwdArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 struct WattnBwdPlan {
-  int nqp, nsb, nch;
-  int64_t stats, part;  // elements of each of lse2 and delta; of the sink tiles' parts
+  int nqp, nsb, nx, per, keep;
+  int64_t stats, part;  // elements of each of lse2 and delta; of the sinks' parts
 };
 
 inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
@@ -475,66 +503,66 @@ inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
   p.stats = static_cast<int64_t>(a.B) * a.Hq * p.nqp;
   const int group = a.Hq / a.Hkv;
   p.nsb = (a.sinks + 127) / 128;
-  const int64_t all = group * ((Nq + 63) / 64);
-  int64_t own = static_cast<int64_t>(a.left) + a.right + 128;
-  own = group * ((own + 63) / 64);
-  if (own < 8) own = 8;
-  int64_t nch = p.nsb > 0 ? (all + own - 1) / own : 1;
-  p.nch = static_cast<int>(nch < 1 ? 1 : nch > 64 ? 64 : nch);
-  if (p.nch == 1) p.nsb = 0;
+  p.keep = a.sinks < 128 ? a.sinks : 128;
+  // queries past the first tile's window, in tiles of 64; a block takes a quarter of a tile's own walk
+  const int64_t last = a.Nk - 1 < 127 ? a.Nk - 1 : 127;
+  int64_t late = last + a.left + 1 - (a.Nk - Nq);
+  late = late < 0 ? 0 : late > Nq ? Nq : late;
+  const int64_t blocks = p.nsb > 0 && late < Nq ? (Nq - late / 8 * 8 + 63) / 64 : 0;
+  const int64_t own = group * ((static_cast<int64_t>(a.left) + a.right + 128 + 63) / 64);
+  p.per = static_cast<int>(own / 4 < 4 ? 4 : own / 4);
+  p.nx = static_cast<int>((blocks + p.per - 1) / p.per);
+  if (p.nx == 0) p.nsb = 0;
   const int64_t DT = a.D <= 64 ? 64 : 128;
-  p.part = p.nsb > 0 ? static_cast<int64_t>(a.B) * a.Hkv * p.nsb * p.nch * 2 * 128 * DT : 0;
+  p.part = static_cast<int64_t>(a.B) * a.Hkv * p.nsb * (1 + static_cast<int64_t>(group) * p.nx) * 2 * p.keep * DT;
   return p;
 }
 
 template <typename T, int DT>
 int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
                           const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
+  bind_context();
   const WattnBwdPlan p = wattn_bwd_plan(a, a.Nq);
   float *lse2 = ws, *delta = ws + p.stats;
   if (a.Hq > 65535 || a.B > 65535) return TOPS_ERR_SHAPE;
-  wattn_stats_kernel<T><<<dim3((p.nqp + 31) / 32, a.Hq, a.B), 256, 0, st>>>(
-      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
-  CUtensorMap q128, k128, v128, d128, q64, k64, v64, d64;
-  if (!wattn_map(&q128, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 128) ||
-      !wattn_map(&d128, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 128) ||
-      !wattn_map(&k128, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 128) ||
-      !wattn_map(&v128, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 128) ||
-      !wattn_map(&q64, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 64) ||
-      !wattn_map(&d64, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 64) ||
-      !wattn_map(&k64, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 64) ||
-      !wattn_map(&v64, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64))
+  CUtensorMap mq, mk, mv, md;
+  if (!wattn_map(&mq, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 64) ||
+      !wattn_map(&md, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 64) ||
+      !wattn_map(&mk, dtype, a.k, a.ks, a.B, a.Nk, a.Hkv, a.D, 64) ||
+      !wattn_map(&mv, dtype, a.v, a.vs, a.B, a.Nk, a.Hkv, a.D, 64))
     return TOPS_ERR_TMAP;
   WattnBwdArgs f;
   f.Nq = a.Nq, f.Nk = a.Nk, f.Hq = a.Hq, f.Hkv = a.Hkv, f.group = a.Hq / a.Hkv, f.D = a.D;
   f.left = a.left, f.right = a.right, f.sinks = a.sinks;
-  f.nsb = p.nsb, f.nch = p.nch, f.nqp = p.nqp, f.mask = a.mask;
+  f.nsb = p.nsb, f.nx = p.nx, f.per = p.per, f.keep = p.keep, f.nqp = p.nqp, f.mask = a.mask;
   f.c = a.scale * kLog2e, f.scale = a.scale, f.lse2 = lse2, f.delta = delta;
   f.part = ws + 2 * p.stats;
+  const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
+  const int kv_tiles = (a.Nk + 127) / 128, q_tiles = (a.Nq + 127) / 128;
+  const int64_t own = heads * kv_tiles, kv_grid = own + heads * p.nsb * f.group * p.nx;
+  const int64_t q_grid = static_cast<int64_t>(q_tiles) * a.Hq * a.B;
+  if (kv_grid >= (int64_t(1) << 31) || q_grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  if (p.nsb > 0 && (heads > 65535 || p.nsb > 32767)) return TOPS_ERR_SHAPE;
   const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
+  wattn_stats_kernel<T, DT><<<dim3((p.nqp + 31) / 32, a.Hq, a.B), 256, 0, st>>>(
+      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
   {
-    f.tiles = (a.Nk + 127) / 128;
-    f.d1 = dv, f.d2 = dk;
-    const int64_t grid = (static_cast<int64_t>(f.nsb) * f.nch + f.tiles - f.nsb) * a.Hkv * a.B;
-    if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+    f.tiles = kv_tiles, f.own = static_cast<int>(own), f.d1 = dv, f.d2 = dk;
     auto kern = wattn_backward_kernel<T, DT, true>;
-    set_smem(kern, smem);
-    kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(k128, v128, q64, d64, f);
-    if (const int rc = launch_status()) return rc;
+    static std::atomic<uint64_t> done{0};
+    set_smem_once(kern, smem, done);
+    kern<<<static_cast<unsigned>(kv_grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mk, mv, mq, md, f);
     if (f.nsb > 0) {
       constexpr int ROWS = 256 / (DT / 8);
-      if (static_cast<int64_t>(a.B) * a.Hkv > 65535 || f.nsb > 32767) return TOPS_ERR_SHAPE;
-      wattn_parts_kernel<T, DT><<<dim3(128 / ROWS, 2 * f.nsb, a.B * a.Hkv), 256, 0, st>>>(f);
-      if (const int rc = launch_status()) return rc;
+      wattn_parts_kernel<T, DT>
+          <<<dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256, 0, st>>>(f);
     }
   }
-  f.tiles = (a.Nq + 127) / 128;
-  f.d1 = dq, f.d2 = nullptr;
-  const int64_t grid = static_cast<int64_t>(f.tiles) * a.Hq * a.B;
-  if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  f.tiles = q_tiles, f.own = 0, f.d1 = dq, f.d2 = nullptr;
   auto kern = wattn_backward_kernel<T, DT, false>;
-  set_smem(kern, smem);
-  kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(q128, d128, k64, v64, f);
+  static std::atomic<uint64_t> done{0};
+  set_smem_once(kern, smem, done);
+  kern<<<static_cast<unsigned>(q_grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mq, md, mk, mv, f);
   return launch_status();
 }
 

@@ -356,7 +356,8 @@ int launch_wattn_decode(const WattnArgs& a, int64_t window, void* out, float* pa
   if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   const size_t smem = sizeof(WattnDecodeSmem<DT>);
   auto kern = wattn_decode_kernel<T, DT>;
-  set_smem(kern, smem);
+  static std::atomic<uint64_t> done{0};
+  set_smem_once(kern, smem, done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(32 * kDecWarps);

@@ -111,11 +111,11 @@ def forward(q, k, v, *, window, sinks=0, scale=None, mask=None, out=None):
     m = _mask(mask, B, Nk, dev)
     q, k, v = _tiles(q), _tiles(k), _tiles(v)
     if out is None:
-        out = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         assert out.shape == (B, Nq, Hq, D) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev, \
             "out must be like q, contiguous"
-    lse = torch.empty((B, Hq, Nq), dtype=torch.float32, device=dev)
+    lse = q.new_empty((B, Hq, Nq), dtype=torch.float32)
     _lib.launch("tops_window_attn_forward", dev, dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 _strides(q, k, v), None if m is None else m.data_ptr(), left, right, int(sinks),
                 D ** -0.5 if scale is None else float(scale), out.data_ptr(), lse.data_ptr())
@@ -139,13 +139,13 @@ def backward(dout, q, k, v, out, lse, *, window, sinks=0, scale=None, mask=None)
     m = _mask(mask, B, Nk, dev)
     q, k, v, dout = _tiles(q), _tiles(k), _tiles(v), _tiles(dout)
     out, lse = out.contiguous(), lse.contiguous()
-    dq = torch.empty((B, Nq, Hq, D), dtype=q.dtype, device=dev)
-    dk = torch.empty((B, Nk, Hkv, D), dtype=q.dtype, device=dev)
+    dq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    dk = torch.empty_like(k, memory_format=torch.contiguous_format)
     dv = torch.empty_like(dk)
     need = ctypes.c_int64(0)
     _lib.call("tops_window_attn_backward_workspace_bytes", dt, B, Nq, Nk, Hq, Hkv, D, left, right, int(sinks),
               ctypes.byref(need))
-    ws = torch.empty(max(16, need.value), dtype=torch.uint8, device=dev)
+    ws = q.new_empty(max(16, need.value), dtype=torch.uint8)
     _lib.launch("tops_window_attn_backward", dev, dt, B, Nq, Nk, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 _strides(q, k, v), None if m is None else m.data_ptr(), left, right, int(sinks),
                 D ** -0.5 if scale is None else float(scale), dout.data_ptr(), _I3(*dout.stride()[:3]),
@@ -177,11 +177,11 @@ def decode(q, k_cache, v_cache, lengths, *, window, sinks=0, scale=None):
     q, k, v = _rows(q), _rows(k_cache), _rows(v_cache)
     if lengths.dtype != torch.int32 or not lengths.is_contiguous():
         lengths = lengths.to(torch.int32).contiguous()
-    out = torch.empty((B, Hq, D), dtype=q.dtype, device=dev)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     need = ctypes.c_int64(0)
     _lib.call("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, window, sinks, ctypes.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=dev).data_ptr() if need.value else None
+    ws = q.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _lib.launch("tops_window_attn_decode", dev, dt, B, N, Hq, Hkv, D, q.data_ptr(), k.data_ptr(), v.data_ptr(),
                 _I8(*q.stride()[:2], *k.stride()[:3], *v.stride()[:3]), lengths.data_ptr(), window, sinks,
-                D ** -0.5 if scale is None else float(scale), ws, out.data_ptr())
+                D ** -0.5 if scale is None else float(scale), None if ws is None else ws.data_ptr(), out.data_ptr())
     return out
