@@ -1,9 +1,12 @@
-"""Build recipe for the in-tree C-ABI library ``libtriangleops_b200.so``.
+"""Build recipe for the in-tree C-ABI library ``libtriangleops_b200.so`` and the
+Python extension ``_bind.so`` on top of it.
 
 The whole CUDA side is one translation unit (``csrc/tops_all.cu``) compiled for
 sm_100a only. ``nvcc`` cross-compiles without a GPU, so this runs anywhere the
 CUDA toolkit is installed; the resulting ``.so`` sits next to this file and is
-loaded with ``ctypes`` by :mod:`triangleops_b200._lib`.
+loaded with ``ctypes`` by :mod:`triangleops_b200._lib`. The extension
+(``csrc/bind.cpp``, host code only, against torch's headers) holds the launchers
+of the token block's operators.
 """
 
 from __future__ import annotations
@@ -17,6 +20,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_NAME = "libtriangleops_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+BIND_SRC = os.path.join(CSRC, "bind.cpp")
+BIND_PATH = os.path.join(HERE, "_bind.so")
 
 NVCC_FLAGS = [
     "-gencode",
@@ -54,20 +59,55 @@ def needs_build() -> bool:
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
+def needs_bind() -> bool:
+    if not os.path.exists(BIND_PATH):
+        return True
+    header = os.path.join(HERE, "..", "include", "triangleops_b200.h")
+    t = os.path.getmtime(BIND_PATH)
+    return any(os.path.exists(s) and os.path.getmtime(s) > t for s in (BIND_SRC, header))
+
+
+def _run(cmd: list[str], tmp: str, path: str, verbose: bool) -> None:
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{cmd[0]} failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, path)
+
+
+def build_bind(verbose: bool = False, force: bool = False) -> str:
+    """Compile ``csrc/bind.cpp`` into ``_bind.so``, linked to ``libtriangleops_b200.so``."""
+    build(verbose=verbose)
+    if not force and not needs_bind():
+        return BIND_PATH
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = BIND_PATH + ".tmp"
+    inc = (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"])
+    cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), BIND_SRC, "-o",
+           tmp, f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
+    _run(cmd, tmp, BIND_PATH, verbose)
+    return BIND_PATH
+
+
 def build(verbose: bool = False, force: bool = False, extra_flags: list[str] | None = None) -> str:
     """Compile ``csrc/tops_all.cu`` into ``libtriangleops_b200.so`` (sm_100a)."""
     if not force and not needs_build():
         return LIB_PATH
     tmp = LIB_PATH + ".tmp"
     cmd = [_nvcc(), *NVCC_FLAGS, *(extra_flags or []), os.path.join(CSRC, "tops_all.cu"), "-o", tmp]
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    os.replace(tmp, LIB_PATH)
+    _run(cmd, tmp, LIB_PATH, verbose)
     return LIB_PATH
 
 
 if __name__ == "__main__":
     print(build(verbose=True, force="--force" in sys.argv))
+    print(build_bind(verbose=True, force="--force" in sys.argv))

@@ -99,23 +99,22 @@ def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args), name)
 
 
-_FN: dict = {}
+_BIND = None
 
 
-def launch(name: str, device: torch.device, *args) -> None:
-    """Call an entry point whose last argument is the stream, on ``device`` and its current
-    stream. The checks and look-ups of :func:`call`, at the cost that a single token allows."""
-    fn = _FN.get(name)
-    if fn is None:
-        fn = _FN[name] = getattr(lib(), name)
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(device):
-            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if code != OK:
-        check(code, name)
+def bind():
+    """Load (building first if its source is newer) and return the extension ``_bind``: the
+    launchers whose checks, allocations and calls are native, for operators that a single
+    token calls."""
+    global _BIND
+    if _BIND is None:
+        lib()
+        if _build.needs_bind():
+            _build.build_bind()
+        from . import _bind
+
+        _BIND = _bind
+    return _BIND
 
 
 def dtype_code(dtype: torch.dtype) -> int:

@@ -22,7 +22,7 @@
 //
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
-// end, has lse2 = +inf, so that its P is 0.
+// end, has -lse2 = -inf, so that its P is 0.
 #include "sm100.cuh"
 #include "wattn.h"
 
@@ -38,7 +38,7 @@ struct WattnBwdArgs {
   int nqp;               // row length of lse2 and delta
   const uint8_t* mask;
   float c, scale;
-  const float *lse2, *delta;  // [B][Hq][nqp]
+  const float *lse2, *delta;  // [B][Hq][nqp], negated
   void *d1, *d2;              // KV: dv, dk; Q: dq
   float* part;                // [B][Hkv][nsb][1 + group nx][2][keep][DT]
 };
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
       lo = p - a.left;
       hi = min(p + a.right + 1, a.Nk);
       upto = a.sinks;
-      // nqp reaches past the last tile's rows: those hold +inf and 0
+      // nqp reaches past the last tile's rows: those hold -inf and 0
       const int64_t q = (static_cast<int64_t>(walk.b) * a.Hq + walk.head) * a.nqp + at;
       lse2 = a.lse2[q];
       delta = a.delta[q];
@@ -302,55 +302,56 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
           see = bits_below(e - r0) & (~bits_below(f - r0) | bits_below(u - r0)) & kept;
         }
       }
-      const float* s_lse = sm.st[r][0] + 32 * g;
-      const float* s_del = sm.st[r][1] + 32 * g;
+      // x: P. The statistics wait negated, in pairs, 16 bytes a load
+      const ulonglong2* s_lse = reinterpret_cast<const ulonglong2*>(sm.st[r][0] + 32 * g);
+      const ulonglong2* s_del = reinterpret_cast<const ulonglong2*>(sm.st[r][1] + 32 * g);
+      auto pair = [](const uint32_t* v, int i) { return f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])); };
+      auto unpair = [](f2 e, uint32_t* v, int i) {
+        float e0, e1;
+        f2_unpack(e, e0, e1);
+        v[2 * i] = __float_as_uint(e0);
+        v[2 * i + 1] = __float_as_uint(e1);
+      };
       uint32_t pk[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        f2 nl;
-        if constexpr (KV)
-          nl = f2_pack(-s_lse[2 * i], -s_lse[2 * i + 1]);
-        else
-          nl = f2_both(-lse2);
-        float p0, p1;
-        f2_unpack(f2_fma(f2_pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), c2, nl), p0, p1);
-        p0 = ex2_approx(p0);
-        p1 = ex2_approx(p1);
-        if (edge) {
-          const uint32_t w = see >> (2 * i);
-          if (!(w & 1)) p0 = 0.f;
-          if (!(w & 2)) p1 = 0.f;
-        }
-        x[2 * i] = __float_as_uint(p0);
-        x[2 * i + 1] = __float_as_uint(p1);
-        if constexpr (KV) pk[i] = E::pack2(p0, p1);
+      for (int i = 0; i < 16; i += 2) {
+        ulonglong2 n = make_ulonglong2(f2_both(lse2), f2_both(lse2));
+        if constexpr (KV) n = s_lse[i / 2];
+        unpair(f2_fma(pair(x, i), c2, n.x), x, i);
+        unpair(f2_fma(pair(x, i + 1), c2, n.y), x, i + 1);
+      }
+#pragma unroll
+      for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(ex2_approx(__uint_as_float(x[i])));
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!(see >> i & 1)) x[i] = 0u;
       }
       if constexpr (KV) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = E::pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
         tmem_st16(t1, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.p_full[s]);
       }
+      // y: dS
       tmem_ld32(t2, y);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        f2 nd;
-        if constexpr (KV)
-          nd = f2_pack(-s_del[2 * i], -s_del[2 * i + 1]);
-        else
-          nd = f2_both(-delta);
-        float d0, d1;
-        f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1])), nd),
-                         f2_pack(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]))),
-                  d0, d1);
-        if (edge) {  // (what an unseen pair's product holds may be NaN)
-          const uint32_t w = see >> (2 * i);
-          if (!(w & 1)) d0 = 0.f;
-          if (!(w & 2)) d1 = 0.f;
-        }
-        pk[i] = E::pack2(d0, d1);
+      for (int i = 0; i < 16; i += 2) {
+        ulonglong2 n = make_ulonglong2(f2_both(delta), f2_both(delta));
+        if constexpr (KV) n = s_del[i / 2];
+        unpair(f2_mul(f2_add(pair(y, i), n.x), pair(x, i)), y, i);
+        unpair(f2_mul(f2_add(pair(y, i + 1), n.y), pair(x, i + 1)), y, i + 1);
       }
+      if (edge) {  // (what an unseen pair's product holds may be NaN)
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (!(see >> i & 1)) y[i] = 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) pk[i] = E::pack2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
       tmem_st16(t2, pk);
       if (!KV && a.mask && !whole && wq == 0) {
         // T1 of this tile is done: its masked keys' rows may be zeroed for dS k
@@ -420,8 +421,8 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
   if (warp == 1) tmem_dealloc(tbase, 512);
 }
 
-// delta = sum_d dO O and lse2 = lse log2(e) per query, in rows of nqp: queries past Nq, and those
-// that see nothing, get lse2 = +inf and delta = 0. Eight threads a query, 16-byte loads.
+// -delta, delta = sum_d dO O, and -lse2 = -lse log2(e) per query, in rows of nqp: queries past Nq, and
+// those that see nothing, get -inf and 0. Eight threads a query, 16-byte loads.
 template <typename T, int DT>
 __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* __restrict__ dout, int64_t s0,
                                                           int64_t s1, int64_t s2, const T* __restrict__ out,
@@ -456,8 +457,8 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
 #pragma unroll
   for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
   if (part == 0 && i < nqp) {
-    lse2[bh * nqp + i] = v == -INFINITY ? INFINITY : v * kLog2e;
-    delta[bh * nqp + i] = v == -INFINITY ? 0.f : x;
+    lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : -v * kLog2e;
+    delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
   }
 }
 
