@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 256 ? 1 : TPR == 2
   __shared__ float red[TPR > 32 ? 128 : 1];
   const bool has_post = ALL || a.has_post, has_pre = ALL || a.has_pre, gated = ALL || a.gate != nullptr;
   int turn = 0;
-  const int tpr = TPR > 32 ? blockDim.x : TPR > 0 ? TPR : a.tpr;
-  const int t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = blockDim.x / tpr, C = a.C;
+  const int tpr = TPR > 0 ? TPR : a.tpr;
+  const int t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = TPR > 32 ? 1 : blockDim.x / tpr, C = a.C;
   f2 pw[NP], pb[NP], sc[NP], nw[NP], nb[NP];
   gn_weight<T, VEC, V>(a.post_w, a.w_io, t, tpr, C, 1.f, pw);
   gn_weight<T, VEC, V>(a.post_b, a.w_io, t, tpr, C, 0.f, pb);
@@ -326,8 +326,8 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 512 ? 1 : TPR > 25
   const bool has_post = ALL || a.has_post, has_pre = ALL || a.has_pre, gated = ALL || a.gate != nullptr;
   const bool has_dh = ALL || a.dh != nullptr, has_dn = ALL || a.dn != nullptr;
   int turn = 0;
-  const int tpr = TPR > 32 ? blockDim.x : TPR > 0 ? TPR : a.tpr;
-  const int t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = blockDim.x / tpr, C = a.C;
+  const int tpr = TPR > 0 ? TPR : a.tpr;
+  const int t = threadIdx.x % tpr, slot = threadIdx.x / tpr, slots = TPR > 32 ? 1 : blockDim.x / tpr, C = a.C;
   const float inv = 1.f / C;
   ulonglong2* wts = reinterpret_cast<ulonglong2*>(buf);
   if (slot == 0) {

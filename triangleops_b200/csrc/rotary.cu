@@ -30,16 +30,17 @@ struct RotaryArgs {
 
 constexpr int kRotThreads = 256;
 
+// cosine and sine of pos * freq, the angle in half turns of one turn
 __device__ __forceinline__ float2 turn_of(double pos, float freq) {
-  const double a = pos * freq;
-  const double turns = rint(a * 0.15915494309189533577);  // 1 / (2 pi)
+  const double half = pos * freq * 0.31830988618379067154;  // 1 / pi
   float s, c;
-  sincosf(static_cast<float>(fma(turns, -6.283185307179586477, a)), &s, &c);
+  sincospif(static_cast<float>(fma(rint(0.5 * half), -2.0, half)), &s, &c);
   return make_float2(c, s);
 }
 
-// VEC channels of one head at a time as 16 bytes (VEC 1: one by one): the two halves' channels of
-// VEC pairs, or VEC / 2 neighbouring pairs. Block (x, y): tokens x * tok.., share y of the heads.
+// Two pieces of VEC channels of a head at a time, 16 bytes each, one from either half (VEC 1: channel
+// by channel): the two halves' channels of VEC pairs, or VEC neighbouring pairs. Block (x, y): tokens
+// x * tok.., share y of the heads.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
   extern __shared__ float2 cs[];  // [tok][P]
@@ -61,9 +62,9 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
   __syncthreads();
   const uint32_t H = a.Hq + a.Hk, half = a.D / 2;
   const uint32_t h_lo = H * blockIdx.y / gridDim.y, nh = H * (blockIdx.y + 1) / gridDim.y - h_lo;
-  // items of a head: pieces of the first half with their mates in the second, and (odd D) the last
-  // channel; or pieces of neighbouring pairs
-  const uint32_t items = a.interleaved ? (a.D + VEC - 1) / VEC : VEC == 1 ? a.D - half : half / VEC;
+  // items of a head: pieces of the first half with those of the second; channel by channel, with (odd
+  // D) the last one alone, or every channel where its mate is its neighbour
+  const uint32_t items = VEC > 1 ? half / VEC : a.interleaved ? a.D : a.D - half;
   for (uint32_t i = threadIdx.x; i < nt * nh * items; i += kRotThreads) {
     const uint32_t hi = i / items, e = i % items, ti = hi / nh, h = h_lo + hi % nh;
     const uint32_t tok = t0 + ti, b = tok / N, n = tok % N;
@@ -99,27 +100,24 @@ __global__ void __launch_bounds__(kRotThreads) rotary_kernel(RotaryArgs a) {
       };
       Piece p, r;
       p.w = *reinterpret_cast<const uint4*>(src + e * VEC);
+      r.w = *reinterpret_cast<const uint4*>(src + half + e * VEC);
+      auto turn = [&](T& x, T& y, uint32_t f) {
+        if (f >= P) return;
+        const float u = static_cast<float>(x), v = static_cast<float>(y);
+        x = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
+        y = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
+      };
       if (a.interleaved) {
 #pragma unroll
         for (int j = 0; j < VEC; j += 2) {
-          const uint32_t f = (e * VEC + j) / 2;
-          if (f >= P) continue;
-          const float u = static_cast<float>(p.v[j]), v = static_cast<float>(p.v[j + 1]);
-          p.v[j] = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
-          p.v[j + 1] = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
+          turn(p.v[j], p.v[j + 1], (e * VEC + j) / 2);
+          turn(r.v[j], r.v[j + 1], (half + e * VEC + j) / 2);
         }
       } else {
-        r.w = *reinterpret_cast<const uint4*>(src + half + e * VEC);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const uint32_t f = e * VEC + j;
-          if (f >= P) continue;
-          const float u = static_cast<float>(p.v[j]), v = static_cast<float>(r.v[j]);
-          p.v[j] = static_cast<T>(fmaf(u, w[f].x, -(v * w[f].y)));
-          r.v[j] = static_cast<T>(fmaf(v, w[f].x, u * w[f].y));
-        }
-        *reinterpret_cast<uint4*>(dst + half + e * VEC) = r.w;
+        for (int j = 0; j < VEC; ++j) turn(p.v[j], r.v[j], e * VEC + j);
       }
+      *reinterpret_cast<uint4*>(dst + half + e * VEC) = r.w;
       *reinterpret_cast<uint4*>(dst + e * VEC) = p.w;
     }
   }
@@ -161,7 +159,7 @@ extern "C" int tops_rotary(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t 
       return aligned16(p) && aligned16(o) && st[0] % VEC == 0 && st[1] % VEC == 0 && st[2] % VEC == 0;
     };
     const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(shares));
-    if (D % (interleaved ? VEC : 2 * VEC) == 0 && (Hq == 0 || fits(q, q_out, a.qs)) &&
+    if (D % (2 * VEC) == 0 && (Hq == 0 || fits(q, q_out, a.qs)) &&
         (Hk == 0 || fits(k, k_out, a.ks)))
       rotary_kernel<T, VEC><<<grid, kRotThreads, smem, st>>>(a);
     else

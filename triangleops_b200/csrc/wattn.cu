@@ -275,22 +275,26 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
       return true;
     };
 
+    // the key mask, 64 bytes a block, the next block's on their way
+    uint8_t byte[2];
+    auto load_mask = [&](int j) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const int k = blk.key(j) + w * 32 + lane;
+        byte[w] = k < a.Nk ? a.mask[static_cast<int64_t>(b) * a.Nk + k] : 0;
+      }
+    };
+    if (MASK) load_mask(0);
     for (int j = 0; j < blk.n; ++j) {
       const int key = blk.key(j);
       const bool nar = blk.narrow(j);
       uint32_t kept[2];
       bool whole = true;
       if constexpr (MASK) {
-        const uint8_t* mk = a.mask + static_cast<int64_t>(b) * a.Nk;
-        uint8_t byte[2];
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const int k = key + w * 32 + lane;
-          byte[w] = k < a.Nk ? mk[k] : 0;
-        }
         kept[0] = __ballot_sync(0xffffffffu, byte[0] != 0);
         kept[1] = __ballot_sync(0xffffffffu, byte[1] != 0);
         whole = (kept[0] & kept[1]) == 0xffffffffu;
+        if (j + 1 < blk.n) load_mask(j + 1);
       }
       if (!mbar_wait(&sm.s_full[j & 1], (j >> 1) & 1, abort, 510)) { ok = false; break; }
       if (warp == 2 && lane == 0) mbar_arrive(&sm.k_empty[j & 1]);  // q k^T of the block is done

@@ -2,7 +2,7 @@
 //
 // With P = 2^(c S - lse2) from the saved log-sum-exp, delta_i = sum_d dO O and dP = dO v^T:
 //   dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,  dV = P^T dO.
-// Two kernels of one shape: 128 rows stay (two operand tiles A1, A2), tiles of 64 rows stream by
+// Two kinds of block of one shape: 128 rows stay (two operand tiles A1, A2), tiles of 64 rows stream by
 // (B1, B2). Per streamed tile, T1 = A1 B1^T and T2 = A2 B2^T (fp32, TMEM); two softmax warpgroups,
 // each with half of the tile's columns, make P and dS from them and put them back to TMEM rounded
 // to the IO dtype (a product's operands have one type); then
@@ -11,7 +11,7 @@
 // accumulate in TMEM. T1 and T2 have two buffers, so the MMAs of one tile run under the softmax of
 // the other, and each product has a warp of its own to issue it: a thread takes some 90 cycles to
 // issue an MMA, and one thread for all 24 of a tile was what bound the kernel (3.5 k cycles a tile).
-// S and dP are computed in both kernels (7 products for the 5 of one that adds dQ up in memory by
+// S and dP are computed in both (7 products for the 5 of one that adds dQ up in memory by
 // atomics): nothing is added in an order that changes, and dS is not stored.
 //
 // KV walks the query heads of its key head one after the other, so the sum over a shared head's
@@ -31,7 +31,8 @@ namespace tops {
 struct WattnBwdArgs {
   int Nq, Nk, Hq, Hkv, group, D;
   int left, right, sinks;
-  int tiles;             // Q: query tiles; KV: key tiles
+  int q_tiles, tiles;    // query tiles, key tiles
+  int kv_blocks;         // blocks of KV; Q's are behind them
   int own;               // KV: blocks of the tiles themselves; behind them, for the sinks' late queries,
   int nsb, nx, per;      // of nsb tiles and each query head, nx blocks of `per` streamed tiles
   int keep;              // rows of a part
@@ -39,7 +40,7 @@ struct WattnBwdArgs {
   const uint8_t* mask;
   float c, scale;
   const float *lse2, *delta;  // [B][Hq][nqp], negated
-  void *d1, *d2;              // KV: dv, dk; Q: dq
+  void *dq, *dk, *dv;
   float* part;                // [B][Hkv][nsb][1 + group nx][2][keep][DT]
 };
 
@@ -106,9 +107,9 @@ struct WattnWalk {
         total = nqb = min(a.per, (max(0, a.Nq - qlo) + 63) >> 6);
       }
     } else {
-      const int tile = blockIdx.x % a.tiles;
-      head = blockIdx.x / a.tiles % a.Hq;
-      b = blockIdx.x / a.tiles / a.Hq;
+      const int u = blockIdx.x - a.kv_blocks, tile = u % a.q_tiles;
+      head = u / a.q_tiles % a.Hq;
+      b = u / a.q_tiles / a.Hq;
       hk = head / a.group;
       row0 = tile * 128;
       blk = WattnBlocks<6>(row0, a.Nq, a.Nk, a.left, a.right, a.sinks);
@@ -128,10 +129,9 @@ struct WattnWalk {
 };
 
 template <typename T, int DT, bool KV>
-__global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
-    wattn_backward_kernel(const __grid_constant__ CUtensorMap map_a1, const __grid_constant__ CUtensorMap map_a2,
-                          const __grid_constant__ CUtensorMap map_b1, const __grid_constant__ CUtensorMap map_b2,
-                          const WattnBwdArgs a) {  // maps: boxes of 64 rows
+__device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, const CUtensorMap& map_a2,
+                                                     const CUtensorMap& map_b1, const CUtensorMap& map_b2,
+                                                     const WattnBwdArgs& a) {
   using Cfg = WattnBwdCfg<DT>;
   using E = Elem<T>;
   constexpr int NST = Cfg::NST, SUB = Cfg::SUB;
@@ -386,9 +386,9 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
         if (a.nx > 0 && walk.kb < a.nsb && row < min(a.keep, a.sinks - walk.row0))
           part = a.part + ((((static_cast<int64_t>(walk.b) * a.Hkv + walk.hk) * a.nsb + walk.kb) *
                                 (1 + a.group * a.nx) + walk.slot) * 2 + g) * a.keep * DT + row * DT;
-        dst = static_cast<T*>(g == 0 ? a.d1 : a.d2) + ((static_cast<int64_t>(walk.b) * a.Nk + at) * a.Hkv + walk.hk) * a.D;
+        dst = static_cast<T*>(g == 0 ? a.dv : a.dk) + ((static_cast<int64_t>(walk.b) * a.Nk + at) * a.Hkv + walk.hk) * a.D;
       } else {
-        dst = static_cast<T*>(a.d1) + ((static_cast<int64_t>(walk.b) * a.Nq + at) * a.Hq + walk.head) * a.D + col0;
+        dst = static_cast<T*>(a.dq) + ((static_cast<int64_t>(walk.b) * a.Nq + at) * a.Hq + walk.head) * a.D + col0;
       }
       const bool live = at < (KV ? a.Nk : a.Nq) && (!KV || walk.slot == 0);
 #pragma unroll
@@ -419,6 +419,19 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tbase, 512);
+}
+
+// Both kinds of block in one launch, KV's first: Q's fill the SMs that the last KV blocks leave. Maps:
+// boxes of 64 rows.
+template <typename T, int DT>
+__global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
+    wattn_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_d,
+                          const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                          const __grid_constant__ WattnBwdArgs a) {
+  if (static_cast<int>(blockIdx.x) < a.kv_blocks)
+    wattn_backward_block<T, DT, true>(map_k, map_v, map_q, map_d, a);
+  else
+    wattn_backward_block<T, DT, false>(map_q, map_d, map_k, map_v, a);
 }
 
 // -delta, delta = sum_d dO O, and -lse2 = -lse log2(e) per query, in rows of nqp: queries past Nq, and
@@ -484,7 +497,7 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) 
   }
   const float f = which == 0 ? 1.f : a.scale;
   const int64_t b = bh / a.Hkv, hk = bh % a.Hkv;
-  T* dst = static_cast<T*>(which == 0 ? a.d1 : a.d2) + ((b * a.Nk + key) * a.Hkv + hk) * a.D + col;
+  T* dst = static_cast<T*>(which == 0 ? a.dv : a.dk) + ((b * a.Nk + key) * a.Hkv + hk) * a.D + col;
   *reinterpret_cast<uint4*>(dst) = make_uint4(E::pack2(v[0] * f, v[1] * f), E::pack2(v[2] * f, v[3] * f),
                                               E::pack2(v[4] * f, v[5] * f), E::pack2(v[6] * f, v[7] * f));
 }
@@ -539,31 +552,24 @@ int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const
   f.c = a.scale * kLog2e, f.scale = a.scale, f.lse2 = lse2, f.delta = delta;
   f.part = ws + 2 * p.stats;
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
-  const int kv_tiles = (a.Nk + 127) / 128, q_tiles = (a.Nq + 127) / 128;
-  const int64_t own = heads * kv_tiles, kv_grid = own + heads * p.nsb * f.group * p.nx;
-  const int64_t q_grid = static_cast<int64_t>(q_tiles) * a.Hq * a.B;
-  if (kv_grid >= (int64_t(1) << 31) || q_grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  f.tiles = (a.Nk + 127) / 128, f.q_tiles = (a.Nq + 127) / 128;
+  const int64_t own = heads * f.tiles, kv = own + heads * p.nsb * f.group * p.nx;
+  const int64_t grid = kv + static_cast<int64_t>(f.q_tiles) * a.Hq * a.B;
+  if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   if (p.nsb > 0 && (heads > 65535 || p.nsb > 32767)) return TOPS_ERR_SHAPE;
-  const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
+  f.own = static_cast<int>(own), f.kv_blocks = static_cast<int>(kv), f.dq = dq, f.dk = dk, f.dv = dv;
   wattn_stats_kernel<T, DT><<<dim3((p.nqp + 31) / 32, a.Hq, a.B), 256, 0, st>>>(
       a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
-  {
-    f.tiles = kv_tiles, f.own = static_cast<int>(own), f.d1 = dv, f.d2 = dk;
-    auto kern = wattn_backward_kernel<T, DT, true>;
-    static std::atomic<uint64_t> done{0};
-    set_smem_once(kern, smem, done);
-    kern<<<static_cast<unsigned>(kv_grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mk, mv, mq, md, f);
-    if (f.nsb > 0) {
-      constexpr int ROWS = 256 / (DT / 8);
-      wattn_parts_kernel<T, DT>
-          <<<dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256, 0, st>>>(f);
-    }
-  }
-  f.tiles = q_tiles, f.own = 0, f.d1 = dq, f.d2 = nullptr;
-  auto kern = wattn_backward_kernel<T, DT, false>;
+  const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
+  auto kern = wattn_backward_kernel<T, DT>;
   static std::atomic<uint64_t> done{0};
   set_smem_once(kern, smem, done);
-  kern<<<static_cast<unsigned>(q_grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mq, md, mk, mv, f);
+  kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mq, md, mk, mv, f);
+  if (f.nsb > 0) {
+    constexpr int ROWS = 256 / (DT / 8);
+    wattn_parts_kernel<T, DT>
+        <<<dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256, 0, st>>>(f);
+  }
   return launch_status();
 }
 
