@@ -13,12 +13,13 @@ in place (residual adds fused, ending node without a transpose copy);
 ``transition`` is the Pairformer pair transition MLP (one fused kernel).
 Around that trunk, the sequence-local token block, with gradients: ``window_attn``
 (attention over a sliding window and a few first tokens), ``gated_norm`` (the norms around
-a block, its gate and residual scale in one pass) and ``rotary`` (positions on several axes).
+a block, its gate and residual scale in one pass) and ``rotary`` (positions on several axes);
+``local_block`` runs them together.
 All compute runs in hand-written sm_100a kernels behind a C-ABI library
 (``libtriangleops_b200.so``); there is no CPU fallback.
 """
 
-from . import attn_pair_bias, gated_norm, pairformer, rotary, transition, triangle_attn, triangle_mul, window_attn
+from . import attn_pair_bias, gated_norm, local_block, pairformer, rotary, transition, triangle_attn, triangle_mul, window_attn
 from .attn_pair_bias import attention_pair_bias
 from .triangle_attn import triangle_attention
 from .triangle_mul import triangle_multiplicative_update
@@ -29,6 +30,7 @@ __all__ = [
     "attn_pair_bias",
     "attention_pair_bias",
     "gated_norm",
+    "local_block",
     "pairformer",
     "rotary",
     "transition",
