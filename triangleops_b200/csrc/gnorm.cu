@@ -144,12 +144,6 @@ __device__ __forceinline__ void gn_weight(const void* w, int io, int t, int tpr,
   for (int i = 0; i < V / 2; ++i) f[i] = f2_pack(v[2 * i], v[2 * i + 1]);
 }
 
-__device__ __forceinline__ float f2_sum(f2 v) {
-  float a, b;
-  f2_unpack(v, a, b);
-  return a + b;
-}
-
 // Sums of N values over the threads of a row. TPR: threads to a row, side by side in a warp (0: a
 // number that only the launch knows); above 32 the row takes the whole block, and `red` is two
 // buffers of N x 32 floats used in turn, so that one barrier a sum is enough.
@@ -229,7 +223,7 @@ __device__ __forceinline__ float2 gn_stats(const f2* f, int t, int tpr, const Gn
 // are on their way while the present one's are worked on. ALL: both norms and a gate (the launch's
 // flags are then not asked, which some 40 branches a row would).
 template <typename T, int VEC, int TPR, bool ALL>
-__global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 256 ? 1 : TPR == 256 ? 2 : 5)
+__global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 256 ? 1 : TPR == 256 ? 2 : VEC > 1 ? 5 : 4)
     gnorm_forward_kernel(const GnormArgs a) {
   constexpr int V = 8, NP = V / 2;
   __shared__ float red[TPR > 32 ? 128 : 1];
@@ -246,13 +240,17 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 256 ? 1 : TPR == 2
   const int rows = static_cast<int>(a.rows), step = gridDim.x * slots;
   int r = blockIdx.x * slots + slot;
   GnRaw<T, VEC, V> rx = {}, ry = {}, rg = {};
+  int group = -1;  // whose gate rg holds, where tokens share one
   auto load = [&](int row) {  // (a thread without a row works on zeros and keeps up with the others)
     if (row >= rows) return;
     rx.load(gn_row<T>(a.x, row, a.xs), t, tpr, C);
     ry.load(gn_row<T>(a.y, row, a.ys), t, tpr, C);
-    if (gated)
-      rg.load(gn_row<T>(a.gate, a.shared ? static_cast<uint32_t>(row) / static_cast<uint32_t>(a.group_rows) : row, a.gs),
-              t, tpr, C);
+    if (gated && !a.shared) rg.load(gn_row<T>(a.gate, row, a.gs), t, tpr, C);
+    if (gated && a.shared) {
+      const int of = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.group_rows);
+      if (of != group) rg.load(gn_row<T>(a.gate, of, a.gs), t, tpr, C);
+      group = of;
+    }
   };
   load(r);
   for (int r0 = blockIdx.x * slots; r0 < rows; r0 += step, r += step) {
@@ -367,11 +365,12 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 512 ? 1 : TPR > 25
       const int r = r_group + i;
       rx.load(gn_row<T>(a.x, r, a.xs), t, tpr, C);
       ry.load(gn_row<T>(a.y, r, a.ys), t, tpr, C);
-      if (gated) rg.load(gn_row<T>(a.gate, a.shared ? grp : r, a.gs), t, tpr, C);
+      if (gated && !a.shared) rg.load(gn_row<T>(a.gate, r, a.gs), t, tpr, C);
       if (has_dh) rh.load(gn_row<T>(a.dh, r, a.dhs), t, tpr, C);
       if (has_dn) rn.load(gn_row<T>(a.dn, r, a.dns), t, tpr, C);
       st_next = reinterpret_cast<const float4*>(a.stats)[r];
     };
+    if (gated && a.shared) rg.load(gn_row<T>(a.gate, grp, a.gs), t, tpr, C);
     load(i0);
     for (int base = share * slots; base < per; base += step, i0 += step) {
       const bool live = i0 < per;
@@ -553,15 +552,15 @@ inline GnormPlan gnorm_plan(int64_t rows, int64_t gate_rows, int64_t C) {
   const int64_t groups = p.groups = p.shared ? gate_rows : 1;
   const int64_t sms = sm_count();
   // as many blocks as the kernels' launch bounds let the SMs hold
-  auto resident = [&](int threads, bool back) -> int64_t {
+  auto resident = [&](int threads) -> int64_t {
     if (threads > 512) return sms;
     if (threads > 256) return sms * 2;
     if (threads > 128) return sms * 3;
     return sms * (threads == 64 ? 10 : 5);
   };
-  const int64_t need = (rows + p.fwd.slots - 1) / p.fwd.slots, most = resident(p.fwd.threads, false);
+  const int64_t need = (rows + p.fwd.slots - 1) / p.fwd.slots, most = resident(p.fwd.threads);
   p.blocks = need < most ? need : most;
-  const int64_t per = rows / groups, bmost = resident(p.bwd.threads, true);
+  const int64_t per = rows / groups, bmost = resident(p.bwd.threads);
   const int64_t gneed = (per + p.bwd.slots - 1) / p.bwd.slots;
   int64_t splits = bmost / groups;
   if (splits < 1) splits = 1;
@@ -637,7 +636,8 @@ extern "C" int tops_gated_norm_forward(int dtype, int w_dtype, int64_t rows, int
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return gnorm_dispatch<8>(dtype, whole, p.fwd.tpr, [&](auto t, auto w, auto tpr) {
     constexpr int VEC = decltype(w)::value, TPR = decltype(tpr)::value;
-    const unsigned grid = static_cast<unsigned>(p.blocks);
+    const int64_t fit = VEC == 1 && p.fwd.threads == 128 ? int64_t(4) * sm_count() : p.blocks;
+    const unsigned grid = static_cast<unsigned>(p.blocks < fit ? p.blocks : fit);
     if (has_post && has_pre && gate != nullptr)
       gnorm_forward_kernel<decltype(t), VEC, TPR, true><<<grid, p.fwd.threads, 0, st>>>(a);
     else

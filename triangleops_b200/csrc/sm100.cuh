@@ -507,6 +507,11 @@ __device__ __forceinline__ unsigned long long f2_fma(unsigned long long a, unsig
 
 using f2 = unsigned long long;
 __device__ __forceinline__ f2 f2_both(float x) { return f2_pack(x, x); }
+__device__ __forceinline__ float f2_sum(f2 v) {
+  float a, b;
+  f2_unpack(v, a, b);
+  return a + b;
+}
 
 __device__ __forceinline__ uint32_t sw128_off(uint32_t row, uint32_t chunk) {
   return row * 128u + (((chunk ^ (row & 7u)) & 7u) << 4);
