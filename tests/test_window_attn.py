@@ -259,7 +259,8 @@ def _decode_ref(q, k, v, lengths, window, sinks):
 @pytest.mark.parametrize("N,Hq,Hkv,D,window,sinks", [
     (1, 1, 1, 32, 1, 0), (40, 4, 4, 32, 16, 2), (300, 8, 2, 128, 100, 4), (1000, 6, 2, 64, 2000, 0),
     (1500, 32, 8, 128, 700, 5), (515, 20, 1, 64, 129, 1), (2100, 40, 2, 128, 1, 0), (333, 3, 3, 40, 33, 300),
-    (200, 2, 1, 24, 64, 3), (130, 2, 2, 7, 64, 3),
+    (200, 2, 1, 24, 64, 3), (130, 2, 2, 7, 64, 3), (9000, 8, 2, 128, 9000, 0), (9001, 20, 1, 64, 6000, 7),
+    (5000, 3, 3, 40, 4999, 1), (700, 64, 32, 128, 650, 9),
 ])
 def test_decode(device, dtype, N, Hq, Hkv, D, window, sinks):
     B = 5

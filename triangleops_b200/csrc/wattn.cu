@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
 // ---------------------------------------------------------------------------
 // A thread that has not used its device yet (autograd has threads of its own) has no current context,
 // without which a tensor map cannot be encoded; the first runtime call that needs one makes it.
-inline void bind_context() {
+static void bind_context() {
   static thread_local uint64_t bound = 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -415,7 +415,7 @@ inline void set_smem_once(K kernel, size_t bytes, std::atomic<uint64_t>& done) {
 }
 
 template <typename T, int DT, bool MASK>
-int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float* lse, cudaStream_t st) {
+static int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float* lse, cudaStream_t st) {
   bind_context();
   CUtensorMap mq, mk, mv, mk32, mv32;
   if (!wattn_map(&mq, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 128) ||

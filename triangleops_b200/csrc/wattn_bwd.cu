@@ -533,7 +533,7 @@ inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
 }
 
 template <typename T, int DT>
-int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
+static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
                           const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
   bind_context();
   const WattnBwdPlan p = wattn_bwd_plan(a, a.Nq);

@@ -8,13 +8,13 @@
 // A warp walks over 16 keys at a time without shared memory: K and V go from memory to the
 // registers of the MMA's B operand by 16-byte loads. The order of a contraction's terms and of an
 // output's columns is free as long as both sides agree, so a lane's 8 neighbouring channels of K
-// serve two contraction steps, and its 8 neighbouring channels of V eight output columns tiles:
+// serve two contraction steps, and its 8 neighbouring channels of V eight tiles of output columns:
 //   S: thread (key lane/4, part lane%4) holds channels 32 s + 8 (lane%4) ..+7 of its key
 //   O: thread (column lane/4, keys 2 (lane%4) + {0, 1, 8, 9}) holds channels 64 u + 8 (lane/4) ..+7
 // The next keys are on their way while the present ones are computed.
 //
-// The visible keys of one (sequence, key head) are shared by the 8 warps of a block, by the blocks of
-// a cluster (partial maxima, sums and outputs are joined through distributed shared memory), and, for
+// The visible keys of one (sequence, key head) are shared by the warps of a block, by the blocks of a
+// cluster (partial maxima, sums and outputs are joined through distributed shared memory), and, for
 // few sequences with long windows, by several clusters, whose parts a second kernel joins.
 #include "sm100.cuh"
 #include "wattn.h"
@@ -33,12 +33,10 @@ struct WattnDecodeArgs {
   float* part;  // [units][splits][16][DT + 2]: sums of p v, then the maximum and the sum of p
 };
 
-constexpr int kDecWarps = 8;
-
-template <int DT>
+template <int DT, int NW>
 struct WattnDecodeSmem {
-  float o[kDecWarps][16][DT];
-  float m[kDecWarps][16], l[kDecWarps][16];
+  float o[NW][16][DT];
+  float m[NW][16], l[NW][16];
   float cm[16], cl[16];  // the block's
 };
 
@@ -86,12 +84,13 @@ __device__ __forceinline__ uint4 load_stream(const void* p) {
   return v;
 }
 
-template <typename T, int DT>
-__global__ void __launch_bounds__(32 * kDecWarps, 1) wattn_decode_kernel(const WattnDecodeArgs a) {
+// NW: warps a block; blocks of two share an SM by fours
+template <typename T, int DT, int NW>
+__global__ void __launch_bounds__(32 * NW, NW == 2 ? 4 : 1) wattn_decode_kernel(const WattnDecodeArgs a) {
   using E = Elem<T>;
   constexpr int NS = DT / 32, NU = DT / 64;
   extern __shared__ uint8_t smem_raw[];
-  auto& sm = *reinterpret_cast<WattnDecodeSmem<DT>*>(smem_raw);
+  auto& sm = *reinterpret_cast<WattnDecodeSmem<DT, NW>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t4 = lane & 3;
   const uint32_t cs = cluster_size(), rank = cluster_rank();
   const int cl = blockIdx.x / cs;
@@ -147,7 +146,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) wattn_decode_kernel(const W
   for (int i = 0; i < 8 * NU; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   int tile = first + warp;
   if (tile < last) load_k(tile);
-  for (; tile < last; tile += kDecWarps) {
+  for (; tile < last; tile += NW) {
     uint4 vr[4][NU];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -169,7 +168,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) wattn_decode_kernel(const W
         mma_16816<T>(s[nt], qa[2 * i + 1], kr[nt][i].z, kr[nt][i].w);
       }
     }
-    if (tile + kDecWarps < last) load_k(tile + kDecWarps);
+    if (tile + NW < last) load_k(tile + NW);
     // rows quad (elements 0, 1) and quad + 8 (2, 3); keys 8 nt + 2 t4 + {0, 1}
     const int past = total - tile * 16;
     float mx[2] = {-INFINITY, -INFINITY};
@@ -245,15 +244,15 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) wattn_decode_kernel(const W
                           o[8 * u + e + 3][2 * r + col]);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < rows * DT; i += 32 * kDecWarps) {
+  for (int i = threadIdx.x; i < rows * DT; i += 32 * NW) {
     const int row = i / DT, d = i % DT;
     float top = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) top = fmaxf(top, sm.m[w][row]);
+    for (int w = 0; w < NW; ++w) top = fmaxf(top, sm.m[w][row]);
     float x = 0.f, y = 0.f;
     if (top > -INFINITY)
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) {
+      for (int w = 0; w < NW; ++w) {
         const float f = ex2_approx(sm.m[w][row] - top);
         x = fmaf(sm.o[w][row][d], f, x);
         y = fmaf(sm.l[w][row], f, y);
@@ -267,7 +266,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1) wattn_decode_kernel(const W
   else
     __syncthreads();
   const int count = rows * DT / cs;
-  for (int j = threadIdx.x; j < count; j += 32 * kDecWarps) {
+  for (int j = threadIdx.x; j < count; j += 32 * NW) {
     const int i = rank * count + j, row = i / DT, d = i % DT;
     float top = sm.cm[row], x, y;
     if (cs == 1) {
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(DT) wattn_decode_join_kernel(const WattnDecode
 // host side
 // ---------------------------------------------------------------------------
 struct WattnDecodePlan {
-  int cluster, splits;
+  int warps, cluster, splits;
   int64_t units, part;
 };
 
@@ -328,21 +327,33 @@ inline WattnDecodePlan wattn_decode_plan(int64_t B, int64_t N, int64_t Hq, int64
   const int64_t sms = sm_count(), w = window < N ? window : N, s = sinks < N - w ? sinks : N - w;
   const int64_t tiles = (w + s + 15) / 16;
   p.units = B * Hkv * ((Hq / Hkv + 15) / 16);
+  // Few units: blocks of 8 warps, so that a cluster has 64 (one sequence, 2 key heads, window 1024:
+  // 6.7 us against 7.9 with blocks of 2). Else blocks of 2, four an SM, whose starts and ends overlap
+  // (8 sequences x 8 key heads, window 4096: 27 us against 56; 64 sequences: 192 against 206).
+  p.warps = p.units * 8 < sms ? 8 : 2;
   p.cluster = 1;
   // more blocks while the SMs are not all busy and a warp has a tile to itself, or while the last
   // round of blocks would idle many SMs and there is work enough to share
-  while (p.cluster < 8 && ((p.units * p.cluster < sms && tiles > p.cluster * kDecWarps) ||
-                           (p.units * p.cluster < 6 * sms && tiles >= 8 * p.cluster * kDecWarps)))
+  while (p.cluster < 8 && ((p.units * p.cluster < sms && tiles > p.cluster * p.warps) ||
+                           (p.units * p.cluster < 6 * sms && tiles >= 8 * p.cluster * p.warps)))
     p.cluster *= 2;
+  // Few units with long windows (more than 4 tiles a warp): as many parts as fill the SMs once, joined
+  // by a second kernel. Clusters of 2 then, since those of 8 leave SMs over in every GPC (one sequence,
+  // window 65536: 25 us against 32).
   p.splits = 1;
-  while (p.units * p.cluster * p.splits < sms && tiles > 2 * p.cluster * p.splits * kDecWarps) p.splits *= 2;
+  if (p.warps == 8 && tiles > 4 * 8 * p.warps) {
+    p.cluster = 2;
+    const int64_t room = sms / (p.units * p.cluster), most = tiles / (2 * p.cluster * p.warps);
+    p.splits = static_cast<int>(room < most ? room : most);
+    if (p.splits < 1) p.splits = 1;
+  }
   p.part = p.splits > 1 ? p.units * p.splits * 16 * ((D <= 64 ? 64 : 128) + 2) : 0;
   return p;
 }
 
-template <typename T, int DT>
-int launch_wattn_decode(const WattnArgs& a, int64_t window, void* out, float* part, cudaStream_t st) {
-  const WattnDecodePlan p = wattn_decode_plan(a.B, a.Nk, a.Hq, a.Hkv, a.D, window, a.sinks);
+template <typename T, int DT, int NW>
+static int launch_wattn_decode(const WattnArgs& a, const WattnDecodePlan& p, int64_t window, void* out, float* part,
+                               cudaStream_t st) {
   WattnDecodeArgs f;
   f.N = a.Nk, f.Hq = a.Hq, f.Hkv = a.Hkv, f.group = a.Hq / a.Hkv, f.D = a.D;
   f.window = static_cast<int>(window < a.Nk ? window : a.Nk), f.sinks = a.sinks;
@@ -354,13 +365,13 @@ int launch_wattn_decode(const WattnArgs& a, int64_t window, void* out, float* pa
   if (p.splits > 1 && (part == nullptr || !aligned16(part))) return TOPS_ERR_ARG;
   const int64_t grid = p.units * p.splits * p.cluster;
   if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
-  const size_t smem = sizeof(WattnDecodeSmem<DT>);
-  auto kern = wattn_decode_kernel<T, DT>;
+  const size_t smem = sizeof(WattnDecodeSmem<DT, NW>);
+  auto kern = wattn_decode_kernel<T, DT, NW>;
   static std::atomic<uint64_t> done{0};
   set_smem_once(kern, smem, done);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(32 * kDecWarps);
+  cfg.blockDim = dim3(32 * NW);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -378,8 +389,12 @@ int launch_wattn_decode(const WattnArgs& a, int64_t window, void* out, float* pa
 
 template <typename T>
 int run_wattn_decode(const WattnArgs& a, int64_t window, void* out, float* part, cudaStream_t st) {
-  return a.D <= 64 ? launch_wattn_decode<T, 64>(a, window, out, part, st)
-                   : launch_wattn_decode<T, 128>(a, window, out, part, st);
+  const WattnDecodePlan p = wattn_decode_plan(a.B, a.Nk, a.Hq, a.Hkv, a.D, window, a.sinks);
+  if (p.warps == 8)
+    return a.D <= 64 ? launch_wattn_decode<T, 64, 8>(a, p, window, out, part, st)
+                     : launch_wattn_decode<T, 128, 8>(a, p, window, out, part, st);
+  return a.D <= 64 ? launch_wattn_decode<T, 64, 2>(a, p, window, out, part, st)
+                   : launch_wattn_decode<T, 128, 2>(a, p, window, out, part, st);
 }
 
 // 16-byte rows; strides of zero are fine here
