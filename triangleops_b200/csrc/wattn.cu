@@ -29,7 +29,7 @@ namespace tops {
 
 struct WattnFwdArgs {
   int Nq, Nk, Hq, group, D;  // group: query heads to a key head
-  int left, right, sinks, tiles;
+  int left, right, sinks, tiles, units;  // units: (tile of queries, head, sequence)
   const uint8_t* mask;
   float c;  // scale * log2(e)
   void* out;
@@ -53,7 +53,7 @@ struct WattnFwdSmem {
   alignas(1024) uint8_t q[Cfg::Q_TILE];
   alignas(1024) uint8_t k[Cfg::NS][Cfg::TILE];
   alignas(1024) uint8_t v[Cfg::NS][Cfg::TILE];
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2];
+  uint64_t q_full, q_empty, o_empty, k_full[2], k_empty[2], v_full[2];
   uint64_t s_full[2], p_full[2], pv_done[2];  // of block j at j & 1
   uint32_t tmem_base;
   int abort;
@@ -93,21 +93,17 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
                          const __grid_constant__ CUtensorMap map_v32, const WattnFwdArgs a) {
   using Cfg = WattnFwdCfg<DT>;
   using E = Elem<T>;
-  constexpr int NS = Cfg::NS, SUB = Cfg::SUB;
+  constexpr int SUB = Cfg::SUB;
   extern __shared__ uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<WattnFwdSmem<DT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
 
-  const int tile = blockIdx.x % a.tiles;
-  const int h = blockIdx.x / a.tiles % a.Hq;
-  const int b = blockIdx.x / a.tiles / a.Hq;
-  const int q0 = tile * 128;
-  const WattnBlocks<6> blk(q0, a.Nq, a.Nk, a.left, a.right, a.sinks);
-
   if (threadIdx.x == 0) {
     mbar_init(&sm.q_full, 1);
-    for (int s = 0; s < NS; ++s) {
+    mbar_init(&sm.q_empty, 1);
+    mbar_init(&sm.o_empty, 4);
+    for (int s = 0; s < Cfg::NS; ++s) {
       mbar_init(&sm.k_full[s], 1);
       mbar_init(&sm.k_empty[s], 1);
       mbar_init(&sm.v_full[s], 1);
@@ -129,80 +125,121 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
   tc_fence_after();
   const uint32_t tbase = sm.tmem_base;
 
+  // Persistent: a CTA takes units blockIdx.x, + gridDim.x, .. Blocks of keys are counted on across
+  // units (g: block j of unit lu is block g + j), so loads and S of the next unit run under the end
+  // of the present one.
+  auto unit = [&](int u, int& tile, int& h, int& b) {
+    tile = u % a.tiles;
+    h = u / a.tiles % a.Hq;
+    b = u / a.tiles / a.Hq;
+  };
+  auto blocks = [&](int tile) { return WattnBlocks<6>(tile * 128, a.Nq, a.Nk, a.left, a.right, a.sinks); };
+  int g = 0, lu = 0;
+
   if (warp == 0) {
     if (lane == 0) {
-      const int hk = h / a.group;
-      auto load = [&](const CUtensorMap* m, uint8_t* dst, uint64_t* bar, int head, int row, int rows, int sub) {
-        mbar_expect_tx(bar, SUB * rows * 128);
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+        int tile, h, b;
+        unit(u, tile, h, b);
+        const WattnBlocks<6> blk = blocks(tile);
+        const int hk = h / a.group;
+        auto load = [&](const CUtensorMap* m, uint8_t* dst, uint64_t* bar, int head, int row, int rows, int sub) {
+          mbar_expect_tx(bar, SUB * rows * 128);
 #pragma unroll
-        for (int s = 0; s < SUB; ++s) tma_load_4d(dst + s * sub, m, bar, s * 64, head, row, b);
-      };
-      load(&map_q, sm.q, &sm.q_full, h, q0, 128, 128 * 128);
-      for (int j = 0; j < blk.n; ++j) {
-        const int s = j % NS;
-        const uint32_t ph = ((j / NS) & 1) ^ 1;
-        const bool nar = blk.narrow(j);
-        const int rows = nar ? 32 : Cfg::BK;
-        if (!mbar_wait(&sm.k_empty[s], ph, abort, 501)) break;
-        load(nar ? &map_k32 : &map_k, sm.k[s], &sm.k_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
-        if (!mbar_wait(&sm.pv_done[s], ph, abort, 502)) break;  // P v of the block before in this stage
-        load(nar ? &map_v32 : &map_v, sm.v[s], &sm.v_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
+          for (int s = 0; s < SUB; ++s) tma_load_4d(dst + s * sub, m, bar, s * 64, head, row, b);
+        };
+        if (!mbar_wait(&sm.q_empty, (lu & 1) ^ 1, abort, 516)) break;  // the unit before has no more S
+        load(&map_q, sm.q, &sm.q_full, h, tile * 128, 128, 128 * 128);
+        for (int j = 0; j < blk.n; ++j, ++g) {
+          const int s = g & 1;
+          const uint32_t ph = ((g >> 1) & 1) ^ 1;
+          const bool nar = blk.narrow(j);
+          const int rows = nar ? 32 : Cfg::BK;
+          ok = mbar_wait(&sm.k_empty[s], ph, abort, 501);
+          if (!ok) break;
+          load(nar ? &map_k32 : &map_k, sm.k[s], &sm.k_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
+          ok = mbar_wait(&sm.pv_done[s], ph, abort, 502);  // P v of the block before in this stage
+          if (!ok) break;
+          load(nar ? &map_v32 : &map_v, sm.v[s], &sm.v_full[s], hk, blk.key(j), rows, Cfg::BK * 128);
+        }
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      // S of block j; its buffer held P of block j - 2
+      // S of block g; its buffer held P of block g - 2
       const int ksteps = (a.D + 15) >> 4;
       const uint32_t qa = smem_u32(sm.q);
-      bool ok = mbar_wait(&sm.q_full, 0, abort, 504);
-      for (int j = 0; ok && j < blk.n; ++j) {
-        const int s = j & 1;
-        if (!mbar_wait(&sm.k_full[s], (j >> 1) & 1, abort, 503)) break;
-        if (!mbar_wait(&sm.pv_done[s], ((j >> 1) & 1) ^ 1, abort, 505)) break;
-        tc_fence_after();
-        const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : Cfg::BK, E::kFmt, false, false);
-        const uint32_t ka = smem_u32(sm.k[s]);
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+        int tile, h, b;
+        unit(u, tile, h, b);
+        const WattnBlocks<6> blk = blocks(tile);
+        if (!mbar_wait(&sm.q_full, lu & 1, abort, 504)) break;
+        for (int j = 0; j < blk.n; ++j, ++g) {
+          const int s = g & 1;
+          ok = mbar_wait(&sm.k_full[s], (g >> 1) & 1, abort, 503) &&
+               mbar_wait(&sm.pv_done[s], ((g >> 1) & 1) ^ 1, abort, 505);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : Cfg::BK, E::kFmt, false, false);
+          const uint32_t ka = smem_u32(sm.k[s]);
 #pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk)
-          if (kk < ksteps)
-            mma_ss(tbase + s * 64, make_smem_desc(qa + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
-                   make_smem_desc(ka + (kk / 4) * Cfg::BK * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
-        mma_commit(&sm.s_full[s]);
+          for (int kk = 0; kk < DT / 16; ++kk)
+            if (kk < ksteps)
+              mma_ss(tbase + s * 64, make_smem_desc(qa + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
+                     make_smem_desc(ka + (kk / 4) * Cfg::BK * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
+          mma_commit(&sm.s_full[s]);
+        }
+        mma_commit(&sm.q_empty);
       }
     }
   } else if (warp == 6) {
     if (lane == 0) {
       const uint32_t idesc_pv = make_idesc_f16(128, DT, E::kFmt, false, true);
-      for (int j = 0; j < blk.n; ++j) {
-        const int s = j & 1;
-        if (!mbar_wait(&sm.v_full[s], (j >> 1) & 1, abort, 506)) break;
-        if (!mbar_wait(&sm.p_full[s], (j >> 1) & 1, abort, 507)) break;
-        tc_fence_after();
-        const uint32_t va = smem_u32(sm.v[s]);
-        const int steps = blk.narrow(j) ? 2 : 4;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+        int tile, h, b;
+        unit(u, tile, h, b);
+        const WattnBlocks<6> blk = blocks(tile);
+        for (int j = 0; j < blk.n; ++j, ++g) {
+          const int s = g & 1;
+          ok = mbar_wait(&sm.v_full[s], (g >> 1) & 1, abort, 506) &&
+               mbar_wait(&sm.p_full[s], (g >> 1) & 1, abort, 507) &&
+               // the first product overwrites O: the unit before must have read it
+               (j > 0 || lu == 0 || mbar_wait(&sm.o_empty, (lu - 1) & 1, abort, 517));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t va = smem_u32(sm.v[s]);
+          const int steps = blk.narrow(j) ? 2 : 4;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          if (kk < steps)
-            mma_ts(tbase + Cfg::O_COL, tbase + s * 64 + kk * 8,
-                   make_smem_desc(va + kk * 2048, Cfg::BK * 128, 1024, kSw128), idesc_pv, j > 0 || kk > 0);
-        mma_commit(&sm.pv_done[s]);
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk < steps)
+              mma_ts(tbase + Cfg::O_COL, tbase + s * 64 + kk * 8,
+                     make_smem_desc(va + kk * 2048, Cfg::BK * 128, 1024, kSw128), idesc_pv, j > 0 || kk > 0);
+          mma_commit(&sm.pv_done[s]);
+        }
       }
     }
   } else {
     const int wq = warp & 3;
     const int row = wq * 32 + lane;  // TMEM lane = query row of the tile
     const uint32_t lane_addr = tbase + (static_cast<uint32_t>(wq * 32) << 16);
+    const float c = a.c, grow = 8.0f / c;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+    int tile, h, b;
+    unit(u, tile, h, b);
+    const WattnBlocks<6> blk = blocks(tile);
     const int p = blk.p0 + row;
     const int lo = p - a.left, hi = min(p + a.right + 1, a.Nk);  // window keys [lo, hi)
-    const float c = a.c, grow = 8.0f / c;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
 
     // One block of NCOL keys; EDGE: some of them may not be seen.
     auto work = [&](auto ncol_c, auto edge_c, int j, int key, const uint32_t* kept) {
       constexpr int NCOL = decltype(ncol_c)::value;
       constexpr bool EDGE = decltype(edge_c)::value;
-      const uint32_t s_addr = lane_addr + (j & 1) * 64;
+      const uint32_t s_addr = lane_addr + ((g + j) & 1) * 64;
       uint32_t x[NCOL];
       if constexpr (NCOL == 64)
         tmem_ld64(s_addr, x);
@@ -235,7 +272,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
         const float mn = need ? mx : m;
         if (j > 0) {
           // O is stable once P v of the block before is done
-          if (!mbar_wait(&sm.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1, abort, 508)) return false;
+          if (!mbar_wait(&sm.pv_done[(g + j - 1) & 1], ((g + j - 1) >> 1) & 1, abort, 508)) return false;
           tc_fence_after();
           const float f = need ? ex2_approx((m - mn) * c) : 1.0f;
           l *= f;
@@ -286,7 +323,8 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     };
     if (MASK) load_mask(0);
     for (int j = 0; j < blk.n; ++j) {
-      const int key = blk.key(j);
+      const int key = blk.key(j), s = (g + j) & 1;
+      const uint32_t ph = ((g + j) >> 1) & 1;
       const bool nar = blk.narrow(j);
       uint32_t kept[2];
       bool whole = true;
@@ -296,8 +334,8 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
         whole = (kept[0] & kept[1]) == 0xffffffffu;
         if (j + 1 < blk.n) load_mask(j + 1);
       }
-      if (!mbar_wait(&sm.s_full[j & 1], (j >> 1) & 1, abort, 510)) { ok = false; break; }
-      if (warp == 2 && lane == 0) mbar_arrive(&sm.k_empty[j & 1]);  // q k^T of the block is done
+      if (!mbar_wait(&sm.s_full[s], ph, abort, 510)) { ok = false; break; }
+      if (warp == 2 && lane == 0) mbar_arrive(&sm.k_empty[s]);  // q k^T of the block is done
       tc_fence_after();
       // every row sees the whole block: up to the first row's end, from the last row's start
       const bool inside = key + Cfg::BK <= min(blk.p0 + a.right + 1, a.Nk) && !blk.sink(j) &&
@@ -311,48 +349,58 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
       if constexpr (MASK) {
         if (!whole) {
           // masked keys' rows of V: zero (the swizzle moves 16-byte chunks within a row only)
-          if (!mbar_wait(&sm.v_full[j % NS], (j / NS) & 1, abort, 511)) { ok = false; break; }
+          if (!mbar_wait(&sm.v_full[s], ph, abort, 511)) { ok = false; break; }
           const uint32_t word = wq & 1 ? kept[1] : kept[0];
           if (row < (nar ? 32 : 64) && !(word >> lane & 1)) {
 #pragma unroll
-            for (int s = 0; s < SUB; ++s)
+            for (int e = 0; e < SUB; ++e)
 #pragma unroll
               for (int i = 0; i < 8; ++i)
-                reinterpret_cast<uint4*>(sm.v[j % NS] + s * Cfg::BK * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sm.v[s] + e * Cfg::BK * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full[j & 1]);
+      if (lane == 0) mbar_arrive(&sm.p_full[s]);
     }
     // ---------------- O / l -> out, lse ----------------
-    if (ok && mbar_wait(&sm.pv_done[(blk.n - 1) & 1], ((blk.n - 1) >> 1) & 1, abort, 512)) {
-      tc_fence_after();
-      const int i = q0 + row;
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D;
+    const int e = g + blk.n - 1;  // the unit's last block
+    g += blk.n;
+    if (!ok || !mbar_wait(&sm.pv_done[e & 1], (e >> 1) & 1, abort, 512)) {
+      ok = false;
+      break;
+    }
+    tc_fence_after();
+    const int i = tile * 128 + row;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D;
 #pragma unroll
-      for (int c0 = 0; c0 < DT; c0 += 32) {
-        uint32_t o[32];
-        tmem_ld32(lane_addr + Cfg::O_COL + c0, o);
-        if (i < a.Nq) {
+    for (int c0 = 0; c0 < DT; c0 += 32) {
+      uint32_t o[32];
+      tmem_ld32(lane_addr + Cfg::O_COL + c0, o);
+      if (c0 + 32 == DT) {  // O has been read: the next unit's products may overwrite it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.o_empty);
+      }
+      if (i < a.Nq) {
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t pk[4];
+        for (int v = 0; v < 4; ++v) {
+          uint32_t pk[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float o0 = __uint_as_float(o[8 * v + 2 * e]), o1 = __uint_as_float(o[8 * v + 2 * e + 1]);
-              pk[e] = l == 0.f ? 0u : E::pack2(o0 * inv, o1 * inv);
-            }
-            if (c0 + 8 * v < a.D) *reinterpret_cast<uint4*>(dst + c0 + 8 * v) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+          for (int w = 0; w < 4; ++w) {
+            const float o0 = __uint_as_float(o[8 * v + 2 * w]), o1 = __uint_as_float(o[8 * v + 2 * w + 1]);
+            pk[w] = l == 0.f ? 0u : E::pack2(o0 * inv, o1 * inv);
           }
+          if (c0 + 8 * v < a.D) *reinterpret_cast<uint4*>(dst + c0 + 8 * v) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
         }
       }
-      if (a.lse && i < a.Nq)
-        a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Nq + i] =
-            l == 0.f ? -INFINITY : (fmaf(m, c, log2f(l))) * 0.69314718055994531f;
+    }
+    if (a.lse && i < a.Nq)
+      a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Nq + i] =
+          l == 0.f ? -INFINITY : (fmaf(m, c, log2f(l))) * 0.69314718055994531f;
     }
   }
   tc_fence_before();
@@ -431,8 +479,10 @@ static int launch_wattn_forward(int dtype, const WattnArgs& a, void* out, float*
   f.Nq = a.Nq, f.Nk = a.Nk, f.Hq = a.Hq, f.group = a.Hq / a.Hkv, f.D = a.D;
   f.left = a.left, f.right = a.right, f.sinks = a.sinks, f.tiles = (a.Nq + 127) / 128;
   f.mask = a.mask, f.c = a.scale * kLog2e, f.out = out, f.lse = lse;
-  const int64_t grid = static_cast<int64_t>(f.tiles) * a.Hq * a.B;
-  if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  const int64_t units = static_cast<int64_t>(f.tiles) * a.Hq * a.B, most = 2 * static_cast<int64_t>(sm_count());
+  if (units >= (int64_t(1) << 30)) return TOPS_ERR_SHAPE;
+  f.units = static_cast<int>(units);
+  const int64_t grid = units < most ? units : most;
   const size_t smem = sizeof(WattnFwdSmem<DT>) + 1024;
   auto kern = wattn_forward_kernel<T, DT, MASK>;
   static std::atomic<uint64_t> done{0};
