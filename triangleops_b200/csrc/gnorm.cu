@@ -476,47 +476,48 @@ __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 512 ? 1 : TPR > 25
   leave(anb, 4);
 }
 
-// out[set][c] = sum over n of in[(set_base + n * set_step) ...]: the blocks' partial rows, added
-// in a fixed order. One block takes 32 channels of one set; its 32 warps share
-// the rows, four loads of a thread at a time.
+// out[set][c] = sum over n of in[set * set_step + n * row_step + c]: the blocks' partial rows, added
+// in a fixed order, for the 5 weights and then for the groups of a gate shared by several blocks, in one
+// launch (backward of 3 groups of 1367 rows of 771 channels: 43 us with two, 39 with one).
+// One block takes 32 channels of one set; its 32 warps share the rows, four loads of a thread at a time.
 struct GnReduceArgs {
-  const float* in;
-  int64_t n, row_step, set_step;  // rows to add, distance between them and between sets, in elements
-  int C;
-  void* out[5];                   // a row per set (null: not wanted), or
-  void* rows;                     // all sets' rows one after the other
-  int sets, io;
+  const float *part, *gpart;
+  int64_t n, splits;  // rows to add of a weight and of a group
+  int C, io, first;   // weights in the IO dtype; first set to add: 0, or 5 (no weight's gradient is wanted)
+  void* out[5];       // a weight's gradient (null: not wanted)
+  void* dgate;
 };
 template <typename T>
 __global__ void __launch_bounds__(1024) gnorm_reduce_kernel(const GnReduceArgs a) {
   __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  const int64_t set = blockIdx.y;
-  void* out = a.rows ? a.rows : a.out[set];
+  const int c = blockIdx.x * 32 + lane, C = a.C;
+  const int set = blockIdx.y + a.first;
+  const bool weight = set < 5;
+  void* out = weight ? a.out[set] : a.dgate;
   if (out == nullptr) return;
+  const int64_t grp = set - 5, step = weight ? 5 * C : C, n = weight ? a.n : a.splits;
   float v = 0.f;
-  if (c < a.C) {
-    const float* p = a.in + set * a.set_step + c;
-    const int n = static_cast<int>(a.n);
+  if (c < C) {
+    const float* p = (weight ? a.part + set * C : a.gpart + grp * a.splits * C) + c;
     int i = warp;
     for (; i + 96 < n; i += 128) {
       float u[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) u[k] = p[(i + 32 * k) * a.row_step];
+      for (int k = 0; k < 4; ++k) u[k] = p[(i + 32 * k) * step];
 #pragma unroll
       for (int k = 0; k < 4; ++k) v += u[k];
     }
-    for (; i < n; i += 32) v += p[i * a.row_step];
+    for (; i < n; i += 32) v += p[i * step];
   }
   s[warp][lane] = v;
   __syncthreads();
-  if (warp != 0 || c >= a.C) return;
+  if (warp != 0 || c >= C) return;
   v = 0.f;
 #pragma unroll
   for (int w = 0; w < 32; ++w) v += s[w][lane];
-  const int64_t at = a.rows ? set * a.C + c : c;
-  if (a.io)
+  const int64_t at = weight ? c : grp * C + c;
+  if (a.io || !weight)
     static_cast<T*>(out)[at] = static_cast<T>(v);
   else
     static_cast<float*>(out)[at] = v;
@@ -710,21 +711,14 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
                         return whole ? run(t, integral_constant<int, VEC>(), v, tpr) : run(t, integral_constant<int, 1>(), v, tpr);
                       });
   if (rc != TOPS_OK) return rc;
-  auto reduce = [&](const GnReduceArgs& r) {
-    return by_io_type(dtype, [&](auto t) {
-      gnorm_reduce_kernel<decltype(t)>
-          <<<dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(r.sets)), 1024, 0, st>>>(r);
-      return launch_status();
-    });
-  };
-  if (dpost_w || dpost_b || dres_s || dpre_w || dpre_b) {
-    const GnReduceArgs r = {a.part, p.bblocks, 5 * C, C, a.C, {dpost_w, dpost_b, dres_s, dpre_w, dpre_b}, nullptr, 5,
-                            a.w_io};
-    if ((rc = reduce(r)) != TOPS_OK) return rc;
-  }
-  if (p.gpart && gate != nullptr) {
-    const GnReduceArgs r = {a.gpart, p.splits, C, p.splits * C, a.C, {}, dgate, static_cast<int>(groups), 1};
-    return reduce(r);
-  }
-  return TOPS_OK;
+  const int weights = dpost_w || dpost_b || dres_s || dpre_w || dpre_b ? 5 : 0;
+  const int64_t sets = weights + (a.gpart != nullptr && gate != nullptr ? groups : 0);
+  if (sets == 0) return TOPS_OK;
+  const GnReduceArgs r = {a.part, a.gpart, p.bblocks, p.splits, a.C, a.w_io, 5 - weights,
+                          {dpost_w, dpost_b, dres_s, dpre_w, dpre_b}, dgate};
+  return by_io_type(dtype, [&](auto t) {
+    gnorm_reduce_kernel<decltype(t)>
+        <<<dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(sets)), 1024, 0, st>>>(r);
+    return launch_status();
+  });
 }
