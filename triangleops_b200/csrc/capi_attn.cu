@@ -34,10 +34,10 @@ inline void set_smem(K kernel, size_t bytes) {
 // previous kernel in the stream still runs (from that kernel's pdl_trigger, or its exit
 // when it has none); the kernel orders its reads of that kernel's results with pdl_wait.
 template <typename... KArgs, typename... Args>
-inline void launch_pdl(void (*kernel)(KArgs...), int grid, int block, size_t smem, cudaStream_t st,
+inline void launch_pdl(void (*kernel)(KArgs...), dim3 grid, int block, size_t smem, cudaStream_t st,
                        Args&&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(block);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;

@@ -43,6 +43,7 @@ struct GnormArgs {
   float* part;             // [blocks][5][C]: gradients of post_w, post_b, res_s, pre_w, pre_b
   float* gpart;            // [groups][splits][C], or null where a group has one block
   int splits;              // blocks that share a group
+  int summed;              // a kernel that adds up the parts follows
   int tpr;                 // threads to a row
 };
 
@@ -319,6 +320,7 @@ template <typename T, int VEC, int V, int TPR, bool ALL>
 __global__ void __launch_bounds__(TPR > 32 ? TPR : 128, TPR > 512 ? 1 : TPR > 256 ? 2 : TPR > 128 ? 3 : TPR == 64 ? 10 : 5)
     gnorm_backward_kernel(const GnormArgs a) {
   constexpr int NP = V / 2;
+  if (a.summed) pdl_trigger();
   __shared__ float red[TPR > 32 ? 128 : 1];
   extern __shared__ __align__(16) float buf[];  // weights [4][NP / 2][tpr] of two pairs, then the row slots' sums
   const bool has_post = ALL || a.has_post, has_pre = ALL || a.has_pre, gated = ALL || a.gate != nullptr;
@@ -498,6 +500,7 @@ __global__ void __launch_bounds__(1024) gnorm_reduce_kernel(const GnReduceArgs a
   if (out == nullptr) return;
   const int64_t grp = set - 5, step = weight ? 5 * C : C, n = weight ? a.n : a.splits;
   float v = 0.f;
+  pdl_wait();
   if (c < C) {
     const float* p = (weight ? a.part + set * C : a.gpart + grp * a.splits * C) + c;
     int i = warp;
@@ -685,6 +688,9 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
   a.part = static_cast<float*>(workspace);
   a.gpart = p.gpart ? a.part + p.bblocks * 5 * C : nullptr;
   a.splits = p.splits, a.tpr = p.bwd.tpr;
+  const int weights = dpost_w || dpost_b || dres_s || dpre_w || dpre_b ? 5 : 0;
+  const int64_t sets = weights + (a.gpart != nullptr && gate != nullptr ? groups : 0);
+  a.summed = sets > 0;
   const int vec = dtype == TOPS_F32 ? 4 : p.v, bytes = dtype == TOPS_F32 ? 4 : 2;
   auto fits = [&](const void* q, int64_t stride) { return gn_pieces(q, stride, vec, bytes); };
   const bool whole = fits(x, xs) && fits(y, ys) && fits(gate, gs) && fits(dh, dhs) && fits(dn, dns) && fits(dx, C) &&
@@ -711,14 +717,12 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
                         return whole ? run(t, integral_constant<int, VEC>(), v, tpr) : run(t, integral_constant<int, 1>(), v, tpr);
                       });
   if (rc != TOPS_OK) return rc;
-  const int weights = dpost_w || dpost_b || dres_s || dpre_w || dpre_b ? 5 : 0;
-  const int64_t sets = weights + (a.gpart != nullptr && gate != nullptr ? groups : 0);
   if (sets == 0) return TOPS_OK;
   const GnReduceArgs r = {a.part, a.gpart, p.bblocks, p.splits, a.C, a.w_io, 5 - weights,
                           {dpost_w, dpost_b, dres_s, dpre_w, dpre_b}, dgate};
   return by_io_type(dtype, [&](auto t) {
-    gnorm_reduce_kernel<decltype(t)>
-        <<<dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(sets)), 1024, 0, st>>>(r);
+    launch_pdl(gnorm_reduce_kernel<decltype(t)>,
+               dim3(static_cast<unsigned>((C + 31) / 32), static_cast<unsigned>(sets)), 1024, 0, st, r);
     return launch_status();
   });
 }

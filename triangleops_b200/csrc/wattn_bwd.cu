@@ -163,6 +163,8 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = sm.tmem_base;
+  if (a.nsb > 0) pdl_trigger();
+  pdl_wait();  // the rows' lse2 and delta come from the kernel before this one
 
   if (warp == 0) {
     if (lane == 0 && walk.total > 0) {
@@ -442,6 +444,7 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
                                                           const float* __restrict__ lse, int nqp,
                                                           float* __restrict__ lse2, float* __restrict__ delta) {
   using E = Elem<T>;
+  pdl_trigger();
   const int i = static_cast<int>((blockIdx.x * 256u + threadIdx.x) >> 3), part = threadIdx.x & 7;
   const int h = blockIdx.y, b = blockIdx.z;
   const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
@@ -475,26 +478,42 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
   }
 }
 
-// Adds the parts of the sinks' rows, in order. One block: a (b, key head), tile, output, some rows.
+// Adds the parts of the sinks' rows, in an order of its own. One block: a (b, key head), tile, output and
+// two rows, whose parts SHARES groups of its threads add up.
+template <int DT>
+struct WattnParts {
+  static constexpr int PER = DT / 8, ROWS = 2, SHARES = 256 / PER / ROWS;  // threads a row, 8 channels each
+};
 template <typename T, int DT>
 __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) {
   using E = Elem<T>;
-  constexpr int PER = DT / 8;  // threads a row, 8 channels each
-  constexpr int ROWS = 256 / PER;
-  const int row = blockIdx.x * ROWS + threadIdx.x / PER, col = threadIdx.x % PER * 8;
+  using W = WattnParts<DT>;
+  __shared__ float sum[W::SHARES][W::ROWS * W::PER][9];
+  const int at = threadIdx.x % (W::PER * W::ROWS), share = threadIdx.x / (W::PER * W::ROWS);
+  const int row = blockIdx.x * W::ROWS + at / W::PER, col = at % W::PER * 8;
   const int which = blockIdx.y & 1, kb = blockIdx.y >> 1;
   const int64_t bh = blockIdx.z;
   const int key = kb * 128 + row;
-  if (row >= a.keep || key >= a.sinks || col >= a.D) return;
-  const int n = 1 + a.group * a.nx;
-  const float* p = a.part + ((bh * a.nsb + kb) * n * 2 + which) * a.keep * DT + row * DT + col;
+  const bool live = row < a.keep && key < a.sinks && col < a.D;
+  const int n = live ? 1 + a.group * a.nx : 0;
+  const float* p = a.part + ((bh * a.nsb + kb) * (1 + a.group * a.nx) * 2 + which) * a.keep * DT + row * DT + col;
   float v[8] = {};
+  pdl_wait();
 #pragma unroll 4
-  for (int i = 0; i < n; ++i, p += 2 * a.keep * DT) {
-    const float4 u = *reinterpret_cast<const float4*>(p), w = *reinterpret_cast<const float4*>(p + 4);
+  for (int i = share; i < n; i += W::SHARES) {
+    const float* q = p + static_cast<int64_t>(i) * 2 * a.keep * DT;
+    const float4 u = *reinterpret_cast<const float4*>(q), w = *reinterpret_cast<const float4*>(q + 4);
     v[0] += u.x, v[1] += u.y, v[2] += u.z, v[3] += u.w;
     v[4] += w.x, v[5] += w.y, v[6] += w.z, v[7] += w.w;
   }
+#pragma unroll
+  for (int k = 0; k < 8; ++k) sum[share][at][k] = v[k];
+  __syncthreads();
+  if (share != 0 || !live) return;
+#pragma unroll
+  for (int s = 1; s < W::SHARES; ++s)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] += sum[s][at][k];
   const float f = which == 0 ? 1.f : a.scale;
   const int64_t b = bh / a.Hkv, hk = bh % a.Hkv;
   T* dst = static_cast<T*>(which == 0 ? a.dv : a.dk) + ((b * a.Nk + key) * a.Hkv + hk) * a.D + col;
@@ -564,11 +583,11 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
   auto kern = wattn_backward_kernel<T, DT>;
   static std::atomic<uint64_t> done{0};
   set_smem_once(kern, smem, done);
-  kern<<<static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st>>>(mq, md, mk, mv, f);
+  launch_pdl(kern, static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st, mq, md, mk, mv, f);
   if (f.nsb > 0) {
-    constexpr int ROWS = 256 / (DT / 8);
-    wattn_parts_kernel<T, DT>
-        <<<dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256, 0, st>>>(f);
+    constexpr int ROWS = WattnParts<DT>::ROWS;
+    launch_pdl(wattn_parts_kernel<T, DT>, dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256,
+               0, st, f);
   }
   return launch_status();
 }
