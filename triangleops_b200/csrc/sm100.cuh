@@ -272,6 +272,17 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int M, int N, uint32_t ab_
 // ----------------------------------------------------------------------------
 // tcgen05: MMA / commit
 // ----------------------------------------------------------------------------
+// True in one lane of a converged warp, always the same one. A warp that stays together up to here issues
+// an MMA in a fraction of the 85-odd cycles that a lane takes which a branch has long parted from the rest.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
+}
+// mbar_wait by a whole warp, with one answer for all of its lanes
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int site) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, site));
+}
 // D(tmem) (+)= A(smem desc) * B(smem desc)^T
 __device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {

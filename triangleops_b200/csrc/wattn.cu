@@ -11,13 +11,15 @@
 // their keys; the others run without. Up to 32 left-behind sinks are a block of 32 keys.
 //
 // One warp loads (TMA; keys past the end and channels past D arrive as zeros), one issues the MMAs
-// of S and another those of P v (a thread takes some 85 cycles to issue one of them, and 100 for a
-// commit: one thread for both took 1.9 k cycles a block and was what bound the kernel), four hold
-// the softmax: a thread owns a query row (a TMEM lane), so row maximum and sum need
-// no exchange. S is a fp32 TMEM tile, P takes its place rounded to the IO dtype (the product's
-// operand type; its sum is taken before the rounding), O accumulates in TMEM and is rescaled only
-// when the maximum has grown by 2^8. S has two buffers: q k^T of the next block runs under the
-// softmax of this one. Two CTAs share an SM and its 512 TMEM columns (S 2 x 64, O up to 128 each).
+// of S and another those of P v, all of its lanes together (a lane on its own takes some 85 cycles
+// to issue one: 61 us for 57.7 at 2 x 4096 queries, 16 heads of 128, window 512), four hold the
+// softmax: a thread owns a query row (a TMEM lane), so row maximum and sum need no exchange. S is a
+// fp32 TMEM tile, P takes its place rounded to the IO dtype (the product's operand type; its sum is
+// taken before the rounding), O accumulates in TMEM and is rescaled only when the maximum has grown
+// by 2^8. S has two buffers: q k^T of the next block runs under the softmax of this one. Two CTAs
+// share an SM and its 512 TMEM columns (S 2 x 64, O up to 128 each). CTAs are persistent: the loads
+// and S of the next tile run under the end of the present one (8192 queries, 16 heads, window 1024:
+// 87.5 us with a CTA a tile, 83.6 so).
 //
 // Masked keys: their score is replaced by -inf, and their rows of the V tile are zeroed in shared
 // memory before P v, so that a NaN there does not pass through 0 * NaN.
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
   constexpr int SUB = Cfg::SUB;
   extern __shared__ uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<WattnFwdSmem<DT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
 
   if (threadIdx.x == 0) {
@@ -166,24 +168,24 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // S of block g; its buffer held P of block g - 2
-      const int ksteps = (a.D + 15) >> 4;
-      const uint32_t qa = smem_u32(sm.q);
-      bool ok = true;
-      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
-        int tile, h, b;
-        unit(u, tile, h, b);
-        const WattnBlocks<6> blk = blocks(tile);
-        if (!mbar_wait(&sm.q_full, lu & 1, abort, 504)) break;
-        for (int j = 0; j < blk.n; ++j, ++g) {
-          const int s = g & 1;
-          ok = mbar_wait(&sm.k_full[s], (g >> 1) & 1, abort, 503) &&
-               mbar_wait(&sm.pv_done[s], ((g >> 1) & 1) ^ 1, abort, 505);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : Cfg::BK, E::kFmt, false, false);
-          const uint32_t ka = smem_u32(sm.k[s]);
+    // S of block g; its buffer held P of block g - 2
+    const int ksteps = (a.D + 15) >> 4;
+    const uint32_t qa = smem_u32(sm.q);
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+      int tile, h, b;
+      unit(u, tile, h, b);
+      const WattnBlocks<6> blk = blocks(tile);
+      if (!mbar_wait_warp(&sm.q_full, lu & 1, abort, 504)) break;
+      for (int j = 0; j < blk.n; ++j, ++g) {
+        const int s = g & 1;
+        ok = mbar_wait_warp(&sm.k_full[s], (g >> 1) & 1, abort, 503) &&
+             mbar_wait_warp(&sm.pv_done[s], ((g >> 1) & 1) ^ 1, abort, 505);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t idesc = make_idesc_f16(128, blk.narrow(j) ? 32 : Cfg::BK, E::kFmt, false, false);
+        const uint32_t ka = smem_u32(sm.k[s]);
+        if (elect_lane()) {
 #pragma unroll
           for (int kk = 0; kk < DT / 16; ++kk)
             if (kk < ksteps)
@@ -191,27 +193,29 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
                      make_smem_desc(ka + (kk / 4) * Cfg::BK * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
           mma_commit(&sm.s_full[s]);
         }
-        mma_commit(&sm.q_empty);
+        __syncwarp();
       }
+      if (elect_lane()) mma_commit(&sm.q_empty);
+      __syncwarp();
     }
   } else if (warp == 6) {
-    if (lane == 0) {
-      const uint32_t idesc_pv = make_idesc_f16(128, DT, E::kFmt, false, true);
-      bool ok = true;
-      for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
-        int tile, h, b;
-        unit(u, tile, h, b);
-        const WattnBlocks<6> blk = blocks(tile);
-        for (int j = 0; j < blk.n; ++j, ++g) {
-          const int s = g & 1;
-          ok = mbar_wait(&sm.v_full[s], (g >> 1) & 1, abort, 506) &&
-               mbar_wait(&sm.p_full[s], (g >> 1) & 1, abort, 507) &&
-               // the first product overwrites O: the unit before must have read it
-               (j > 0 || lu == 0 || mbar_wait(&sm.o_empty, (lu - 1) & 1, abort, 517));
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t va = smem_u32(sm.v[s]);
-          const int steps = blk.narrow(j) ? 2 : 4;
+    const uint32_t idesc_pv = make_idesc_f16(128, DT, E::kFmt, false, true);
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, ++lu) {
+      int tile, h, b;
+      unit(u, tile, h, b);
+      const WattnBlocks<6> blk = blocks(tile);
+      for (int j = 0; j < blk.n; ++j, ++g) {
+        const int s = g & 1;
+        ok = mbar_wait_warp(&sm.v_full[s], (g >> 1) & 1, abort, 506) &&
+             mbar_wait_warp(&sm.p_full[s], (g >> 1) & 1, abort, 507) &&
+             // the first product overwrites O: the unit before must have read it
+             (j > 0 || lu == 0 || mbar_wait_warp(&sm.o_empty, (lu - 1) & 1, abort, 517));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t va = smem_u32(sm.v[s]);
+        const int steps = blk.narrow(j) ? 2 : 4;
+        if (elect_lane()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             if (kk < steps)
@@ -219,6 +223,7 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
                      make_smem_desc(va + kk * 2048, Cfg::BK * 128, 1024, kSw128), idesc_pv, j > 0 || kk > 0);
           mma_commit(&sm.pv_done[s]);
         }
+        __syncwarp();
       }
     }
   } else {

@@ -9,8 +9,8 @@
 //   KV: rows are keys (A = k, v; B = q, dO):    dV += P B2,  dK += dS B1
 //   Q : rows are queries (A = q, dO; B = k, v): dQ += dS B1
 // accumulate in TMEM. T1 and T2 have two buffers, so the MMAs of one tile run under the softmax of
-// the other, and each product has a warp of its own to issue it: a thread takes some 90 cycles to
-// issue an MMA, and one thread for all 24 of a tile was what bound the kernel (3.5 k cycles a tile).
+// the other, and each product has a warp of its own to issue it, all of its lanes together (a lane on its
+// own takes some 90 cycles an MMA: 219 us for 204 at 2 x 4096 queries, 16 heads of 128, window 512).
 // S and dP are computed in both (7 products for the 5 of one that adds dQ up in memory by
 // atomics): nothing is added in an order that changes, and dS is not stored.
 //
@@ -137,7 +137,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
   constexpr int NST = Cfg::NST, SUB = Cfg::SUB;
   extern __shared__ uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<WattnBwdSmem<DT>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   volatile int* abort = &sm.abort;
   const WattnWalk<KV> walk(a);
 
@@ -196,45 +196,51 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
   } else if (warp <= 2) {
     // T1 (warp 1) and T2 (warp 2); a buffer is free once the product that read P (KV: T1's) or dS
     // out of it is done. (Q keeps no P: T1's goes with dS.)
-    if (lane == 0 && walk.total > 0) {
+    if (walk.total > 0) {
       const uint32_t idesc = make_idesc_f16(128, 64, E::kFmt, false, false);
       const int ksteps = (a.D + 15) >> 4;
       const uint32_t ra = smem_u32(warp == 1 ? sm.a1 : sm.a2);
       uint64_t* const free = KV && warp == 1 ? sm.p_free : sm.ds_free;
-      bool ok = mbar_wait(&sm.res_full, 0, abort, 523);
+      bool ok = mbar_wait_warp(&sm.res_full, 0, abort, 523);
       for (int it = 0; ok && it < walk.total; ++it) {
         const int r = it % NST, s = it & 1;
-        if (!mbar_wait(&sm.full[r], (it / NST) & 1, abort, 522)) break;
-        if (!mbar_wait(&free[s], ((it >> 1) & 1) ^ 1, abort, 524)) break;
+        if (!mbar_wait_warp(&sm.full[r], (it / NST) & 1, abort, 522)) break;
+        if (!mbar_wait_warp(&free[s], ((it >> 1) & 1) ^ 1, abort, 524)) break;
         tc_fence_after();
         const uint32_t rb = smem_u32(warp == 1 ? sm.b1[r] : sm.b2[r]), t = tbase + s * 128 + (warp - 1) * 64;
+        if (elect_lane()) {
 #pragma unroll
-        for (int kk = 0; kk < DT / 16; ++kk)
-          if (kk < ksteps)
-            mma_ss(t, make_smem_desc(ra + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
-                   make_smem_desc(rb + (kk / 4) * 64 * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
-        mma_commit(&sm.t_full[s]);
+          for (int kk = 0; kk < DT / 16; ++kk)
+            if (kk < ksteps)
+              mma_ss(t, make_smem_desc(ra + (kk / 4) * 128 * 128 + (kk % 4) * 32, 16, 1024, kSw128),
+                     make_smem_desc(rb + (kk / 4) * 64 * 128 + (kk % 4) * 32, 16, 1024, kSw128), idesc, kk > 0);
+          mma_commit(&sm.t_full[s]);
+        }
+        __syncwarp();
       }
     }
   } else if (warp <= 4) {
     // KV: dV += P B2 (warp 3), dK += dS B1 (warp 4); Q: dQ += dS B1 (warp 4)
-    if (lane == 0 && (KV || warp == 4)) {
+    if (KV || warp == 4) {
       const uint32_t idesc = make_idesc_f16(128, DT, E::kFmt, false, true);
       const bool of_p = warp == 3;
       const uint32_t acc = tbase + Cfg::ACC + (KV && !of_p ? DT : 0);
       for (int it = 0; it < walk.total; ++it) {
         const int r = it % NST, s = it & 1;
-        if (!mbar_wait(of_p ? &sm.p_full[s] : &sm.ds_full[s], (it >> 1) & 1, abort, 528)) break;
+        if (!mbar_wait_warp(of_p ? &sm.p_full[s] : &sm.ds_full[s], (it >> 1) & 1, abort, 528)) break;
         tc_fence_after();
         const uint32_t t = tbase + s * 128 + (of_p ? 0 : 64), rb = smem_u32(of_p ? sm.b2[r] : sm.b1[r]);
-        // a warpgroup leaves its 32 columns, packed to 16, where they were: at 0 and 32
+        if (elect_lane()) {
+          // a warpgroup leaves its 32 columns, packed to 16, where they were: at 0 and 32
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_ts(acc, t + (kk >> 1) * 32 + (kk & 1) * 8, make_smem_desc(rb + kk * 2048, 64 * 128, 1024, kSw128), idesc,
-                 it > 0 || kk > 0);
-        mma_commit(of_p ? &sm.p_free[s] : &sm.ds_free[s]);
-        mma_commit(&sm.empty[r]);
-        if (it + 1 == walk.total) mma_commit(&sm.acc_done);
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ts(acc, t + (kk >> 1) * 32 + (kk & 1) * 8, make_smem_desc(rb + kk * 2048, 64 * 128, 1024, kSw128), idesc,
+                   it > 0 || kk > 0);
+          mma_commit(of_p ? &sm.p_free[s] : &sm.ds_free[s]);
+          mma_commit(&sm.empty[r]);
+          if (it + 1 == walk.total) mma_commit(&sm.acc_done);
+        }
+        __syncwarp();
       }
     }
   } else {
