@@ -388,17 +388,24 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
       const int col0 = KV ? 0 : g * COLS;
       const uint32_t acc = lane_addr + Cfg::ACC + (KV ? g * DT : col0);
       float* part = nullptr;
+      int parts = 0;  // rows of the tile whose sums go to the parts
       T* dst;
+      int64_t pitch;
+      const int at0 = walk.row0 + wq * 32;
       if constexpr (KV) {
-        // (a row that only some warps' lanes own: they all load, and store what is theirs)
-        if (a.nx > 0 && walk.kb < a.nsb && row < min(a.keep, a.sinks - walk.row0))
+        if (a.nx > 0 && walk.kb < a.nsb) parts = min(a.keep, a.sinks - walk.row0);
+        if (row < parts)
           part = a.part + ((((static_cast<int64_t>(walk.b) * a.Hkv + walk.hk) * a.nsb + walk.kb) *
                                 (1 + a.group * a.nx) + walk.slot) * 2 + g) * a.keep * DT + row * DT;
-        dst = static_cast<T*>(g == 0 ? a.dv : a.dk) + ((static_cast<int64_t>(walk.b) * a.Nk + at) * a.Hkv + walk.hk) * a.D;
+        pitch = static_cast<int64_t>(a.Hkv) * a.D;
+        dst = static_cast<T*>(g == 0 ? a.dv : a.dk) + (static_cast<int64_t>(walk.b) * a.Nk + at0) * pitch + walk.hk * a.D;
       } else {
-        dst = static_cast<T*>(a.dq) + ((static_cast<int64_t>(walk.b) * a.Nq + at) * a.Hq + walk.head) * a.D + col0;
+        pitch = static_cast<int64_t>(a.Hq) * a.D;
+        dst = static_cast<T*>(a.dq) + (static_cast<int64_t>(walk.b) * a.Nq + at0) * pitch + walk.head * a.D;
       }
-      const bool live = at < (KV ? a.Nk : a.Nq) && (!KV || walk.slot == 0);
+      // rows of this warp that leave for the result itself: [from, to)
+      const int from = max(0, parts - wq * 32), to = KV && walk.slot > 0 ? 0 : (KV ? a.Nk : a.Nq) - at0;
+      uint8_t* buf = sm.a1 + (warp - 5) * 2048;  // (all products that read the tile are done)
 #pragma unroll
       for (int c0 = 0; c0 < COLS; c0 += 32) {
         uint32_t o[32];
@@ -410,17 +417,14 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             *reinterpret_cast<uint4*>(part + c0 + 4 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-        } else if (live) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t pk[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              pk[e] = E::pack2(__uint_as_float(o[8 * v + 2 * e]) * f, __uint_as_float(o[8 * v + 2 * e + 1]) * f);
-            if (col0 + c0 + 8 * v < a.D)
-              *reinterpret_cast<uint4*>(dst + c0 + 8 * v) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-          }
         }
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) pk[e] = E::pack2(__uint_as_float(o[2 * e]) * f, __uint_as_float(o[2 * e + 1]) * f);
+        store_rows(buf, lane, pk, [&](int r, int ch) -> void* {
+          const int col = col0 + c0 + ch;
+          return r >= from && r < to && col < a.D ? dst + r * pitch + col : nullptr;
+        });
       }
     }
   }
