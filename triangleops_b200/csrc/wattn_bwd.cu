@@ -122,6 +122,11 @@ struct WattnWalk {
     if constexpr (KV) return qlo + it % nqb * 64;
     return blk.key(it);
   }
+  // and that of the tile after it (without the division that a walk over several heads takes)
+  __device__ int row_after(int row, int it) const {
+    if constexpr (KV) return row + 64 == qlo + nqb * 64 ? qlo : row + 64;
+    return blk.key(it + 1);
+  }
   __device__ int qhead(int it) const {
     if constexpr (KV) return head + it / nqb;
     return head;
@@ -273,8 +278,10 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
     }
     const f2 c2 = f2_both(a.c);
     bool ok = true;
+    int next = walk.total > 0 ? walk.row(0) : 0;
     for (int it = 0; it < walk.total; ++it) {
-      const int r = it % NST, s = it & 1, r0 = walk.row(it) + 32 * g;  // this warpgroup's first streamed row
+      const int r = it % NST, s = it & 1, r0 = next + 32 * g;  // this warpgroup's first streamed row
+      next = walk.row_after(next, it);
       uint32_t kept = 0xffffffffu;
       bool whole = keep;
       if (!KV && a.mask) {
