@@ -96,6 +96,17 @@ def test_masks(device, dtype, D, kind):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("B,N,Hq,Hkv,D,window,sinks", [(9, 700, 8, 2, 64, 100, 40), (3, 1300, 10, 5, 128, (50, 20), 0),
+                                                       (40, 129, 8, 8, 32, 1, 1)])
+def test_more_tiles_than_blocks(device, dtype, B, N, Hq, Hkv, D, window, sinks):
+    """Blocks that take several tiles, over the ends of heads and sequences, some with no key at all."""
+    mask = torch.rand(B, N, generator=torch.Generator().manual_seed(B)) < 0.8
+    mask[1] = False
+    _check(device, dtype, B, N, N, Hq, Hkv, D, window, sinks, mask.to(device), seed=N)
+
+
+@gpu
 def test_mask_types(device):
     q, k, v, _ = _inputs(device, BF, 2, 90, 90, 2, 2, 64)
     keep = (torch.rand(2, 90, generator=torch.Generator().manual_seed(1)) < 0.5).to(device)
