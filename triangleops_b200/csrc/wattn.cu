@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t bits_below(int n) {
 
 // A warp's 32 rows of 32 channels, lane's row in pk, to where at(row, channel) says (null: nowhere) in
 // 64-byte pieces, through 2 KB of shared memory: a lane that stores its own row writes half a sector of
-// 32 lines at once (2 x 4096 queries, 16 heads of 128, window 512: forward 57.7 us with that, 55.8 so,
+// 32 lines at once (2 x 4096 queries, 16 heads of 128, window 512: forward 57.7 us with that, 55.4 so,
 // backward 204 and 198).
 template <typename F>
 __device__ __forceinline__ void store_rows(uint8_t* buf, int lane, const uint32_t* pk, F&& at) {
@@ -406,23 +406,21 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     T* dst = static_cast<T*>(a.out) + ((static_cast<int64_t>(b) * a.Nq + i0) * a.Hq + h) * a.D;
     const int64_t pitch = static_cast<int64_t>(a.Hq) * a.D;
 #pragma unroll
-    for (int c0 = 0; c0 < DT; c0 += 64) {
-      uint32_t o[64], pk[32];
-      tmem_ld64(lane_addr + Cfg::O_COL + c0, o);
-      if (c0 + 64 == DT) {  // O has been read: the next unit's products may overwrite it
+    for (int c0 = 0; c0 < DT; c0 += 32) {
+      uint32_t o[32], pk[16];
+      tmem_ld32(lane_addr + Cfg::O_COL + c0, o);
+      if (c0 + 32 == DT) {  // O has been read: the next unit's products may overwrite it
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.o_empty);
       }
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
+      for (int e = 0; e < 16; ++e)
         pk[e] = l == 0.f ? 0u : E::pack2(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-#pragma unroll
-      for (int c1 = 0; c1 < 64; c1 += 32)
-        store_rows(sm.o[wq], lane, pk + c1 / 2, [&](int r, int ch) -> void* {
-          const int col = c0 + c1 + ch;
-          return i0 + r < a.Nq && col < a.D ? dst + r * pitch + col : nullptr;
-        });
+      store_rows(sm.o[wq], lane, pk, [&](int r, int ch) -> void* {
+        const int col = c0 + ch;
+        return i0 + r < a.Nq && col < a.D ? dst + r * pitch + col : nullptr;
+      });
     }
     if (a.lse && i < a.Nq)
       a.lse[(static_cast<int64_t>(b) * a.Hq + h) * a.Nq + i] =
