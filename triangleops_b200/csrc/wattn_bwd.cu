@@ -4,16 +4,17 @@
 //   dS = P (dP - delta),  dQ = scale dS k,  dK = scale dS^T q,  dV = P^T dO.
 // Two kinds of block of one shape: 128 rows stay (two operand tiles A1, A2), tiles of 64 rows stream by
 // (B1, B2). Per streamed tile, T1 = A1 B1^T and T2 = A2 B2^T (fp32, TMEM); two softmax warpgroups,
-// each with half of the tile's columns, make P and dS from them and put them back to TMEM rounded
-// to the IO dtype (a product's operands have one type); then
+// each with half of the tile's columns, make P and dS from them and put them back to TMEM in the IO
+// dtype (a product's operands have one type): P rounded, dS as its rounding and the rounding of what
+// that leaves, multiplied one after the other; then
 //   KV: rows are keys (A = k, v; B = q, dO):    dV += P B2,  dK += dS B1
 //   Q : rows are queries (A = q, dO; B = k, v): dQ += dS B1
 // accumulate in TMEM. T1 and T2 have two buffers, so the MMAs of one tile run under the softmax of
 // the other, and each product has a warp of its own to issue it, all of its lanes together (a lane on its
 // own takes some 90 cycles an MMA: 219 us for 204 at 2 x 4096 queries, 16 heads of 128, window 512).
-// Bound by the softmax warps' chain (TMEM load, exponentials, store, barrier): 1.8 k cycles a streamed
-// tile, of which the tensor pipe works some 45 %. 2 x 4096 queries, 16 heads of 128 on 4, window 512, 4 sinks:
-// 194 us with the two small kernels around it, 586 TFLOP/s of its 7 products.
+// Bound by the softmax warps' chain (TMEM load, exponentials, store, barrier): some 2 k cycles a streamed
+// tile, of which the tensor pipe works half. 2 x 4096 queries, 16 heads of 128 on 4, window 512, 4 sinks: 216 us
+// with the two small kernels around it, 676 TFLOP/s of its products, dS's twice.
 // S and dP are computed in both (7 products for the 5 of one that adds dQ up in memory by
 // atomics): nothing is added in an order that changes, and dS is not stored.
 //
@@ -244,6 +245,11 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
           for (int kk = 0; kk < 4; ++kk)
             mma_ts(acc, t + (kk >> 1) * 32 + (kk & 1) * 8, make_smem_desc(rb + kk * 2048, 64 * 128, 1024, kSw128), idesc,
                    it > 0 || kk > 0);
+          if (!of_p)  // what dS's rounding leaves, in the 16 columns behind each
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ts(acc, t + (kk >> 1) * 32 + (kk & 1) * 8 + 16, make_smem_desc(rb + kk * 2048, 64 * 128, 1024, kSw128),
+                     idesc, true);
           mma_commit(of_p ? &sm.p_free[s] : &sm.ds_free[s]);
           mma_commit(&sm.empty[r]);
           if (it + 1 == walk.total) mma_commit(&sm.acc_done);
@@ -371,6 +377,18 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
 #pragma unroll
       for (int i = 0; i < 16; ++i) pk[i] = E::pack2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
       tmem_st16(t2, pk);
+      // dS with twice the dtype's digits: its differences P (dP - delta) cancel in the sums of dQ and dK, and
+      // rounded once they put these 1.5 to 1.8 times as far from the 64-bit values as the results' own
+      // rounding does (bf16: 0.0024 in the 2-norm, so 0.0017). 2 x 4096 queries, window 512: 193 us rounded
+      // once, 216 so; P, which only dV and the forward read, is rounded once (dV: 0.0024).
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const f2 r = f2_fma(f2_pack(E::lo(pk[i]), E::hi(pk[i])), f2_both(-1.f), pair(y, i));
+        float r0, r1;
+        f2_unpack(r, r0, r1);
+        pk[i] = E::pack2(r0, r1);
+      }
+      tmem_st16(t2 + 16, pk);
       if (!KV && a.mask && !whole && wq == 0) {
         // T1 of this tile is done: its masked keys' rows may be zeroed for dS k
         if (!(kept >> lane & 1)) {
