@@ -1,0 +1,35 @@
+"""The token block's operators at the edges of what they take: empty and oversized calls, narrow
+ranges of a type, what nobody sees, and calls that C makes without Python's checks."""
+import ctypes
+
+import pytest
+import torch
+
+import block_refs as ref
+from triangleops_b200 import _lib, window_attn
+
+gpu = pytest.mark.gpu
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _c(name, *args):
+    """The status of a C entry: tensors as their pointers, None as null, lists of int as int64 arrays."""
+    def arg(a):
+        if a is None or isinstance(a, torch.Tensor):
+            return ctypes.c_void_p(_lib.ptr(a))
+        if isinstance(a, list):
+            return (ctypes.c_int64 * len(a))(*a)
+        return ctypes.c_float(a) if isinstance(a, float) else a if not isinstance(a, int) else ctypes.c_int64(a)
+
+    return getattr(_lib.lib(), name)(*map(arg, args))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_no_queries_in_c(device, dtype):
+    """Without queries a C caller has no q, k or v to give: the gradients are zero, nothing is read."""
+    B, Nk, H, D = 2, 9, 2, 64
+    dk, dv = (torch.full((B, Nk, H, D), float("nan"), dtype=dtype, device=device) for _ in range(2))
+    assert _c("tops_window_attn_backward", _lib.dtype_code(dtype), B, 0, Nk, H, H, D, None, None, None, None, None, 3, 0, 0,
+              1.0, None, None, None, None, None, None, dk, dv, ctypes.c_void_p(_lib.stream_ptr())) == _lib.OK
+    assert not dk.any() and not dv.any()

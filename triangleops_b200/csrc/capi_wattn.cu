@@ -77,12 +77,20 @@ extern "C" int tops_window_attn_backward(int dtype, int64_t B, int64_t Nq, int64
   WattnArgs a;
   if (const int rc = wattn_args(a, B, Nq, Nk, Hq, Hkv, D, q, k, v, strides, mask, left, right, sinks, scale)) return rc;
   if (B == 0 || Nk == 0) return TOPS_OK;
-  if (dout_strides == nullptr || workspace == nullptr || dk == nullptr || dv == nullptr) return TOPS_ERR_ARG;
-  if (!aligned16(workspace)) return TOPS_ERR_ALIGN;
-  if (Nq > 0 && (dout == nullptr || out == nullptr || lse == nullptr || dq == nullptr)) return TOPS_ERR_ARG;
+  if (dk == nullptr || dv == nullptr) return TOPS_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (Nq == 0) {  // no query reads a key: nothing else of the call is looked at
+    const size_t bytes = static_cast<size_t>(B) * Nk * Hkv * D * (dtype == TOPS_F32 ? 4 : 2);
+    return cudaMemsetAsync(dk, 0, bytes, st) == cudaSuccess && cudaMemsetAsync(dv, 0, bytes, st) == cudaSuccess
+               ? launch_status()
+               : TOPS_ERR_CUDA;
+  }
+  if (dout_strides == nullptr || workspace == nullptr || dout == nullptr || out == nullptr || lse == nullptr ||
+      dq == nullptr)
+    return TOPS_ERR_ARG;
+  if (!aligned16(workspace)) return TOPS_ERR_ALIGN;
   float* delta = static_cast<float*>(workspace);
-  if (Nq > 0 && wattn_tensor(dtype, a) && wattn_fits(dout, dout_strides, a.B, a.Nq, a.Hq) && aligned16(out) &&
+  if (wattn_tensor(dtype, a) && wattn_fits(dout, dout_strides, a.B, a.Nq, a.Hq) && aligned16(out) &&
       aligned16(dq) && aligned16(dk) && aligned16(dv))
     return dtype == TOPS_BF16
                ? run_wattn_backward<__nv_bfloat16>(dtype, a, dout, dout_strides, out, lse, delta, dq, dk, dv, st)

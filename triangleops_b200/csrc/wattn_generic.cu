@@ -411,7 +411,6 @@ template <typename T>
 int run_wattn_delta(const WattnArgs& a, const void* dout, const int64_t* ds, const void* out, float* delta,
                     cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq * a.Nq;
-  if (rows == 0) return TOPS_OK;
   wattn_delta_kernel<T><<<static_cast<unsigned>((rows + kGenWarps - 1) / kGenWarps), 32 * kGenWarps, 0, st>>>(
       a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), delta);
   return launch_status();
@@ -428,9 +427,8 @@ int run_wattn_generic_backward(const WattnArgs& a, const void* dout, const int64
     constexpr size_t smem_q = gen_smem_bytes(NC, 4, kGenRows), smem_kv = gen_smem_bytes(NC, 4, 2 * kGenRows);
     if (smem_q > 48 * 1024) set_smem(wattn_generic_dq_kernel<T, NC>, smem_q);
     if (smem_kv > 48 * 1024) set_smem(wattn_generic_dkv_kernel<T, NC>, smem_kv);
-    if (rows > 0)
-      wattn_generic_dq_kernel<T, NC><<<static_cast<unsigned>(rows), 32 * kGenWarps, smem_q, st>>>(
-          a, d, ds[0], ds[1], ds[2], lse, delta, static_cast<T*>(dq));
+    wattn_generic_dq_kernel<T, NC><<<static_cast<unsigned>(rows), 32 * kGenWarps, smem_q, st>>>(
+        a, d, ds[0], ds[1], ds[2], lse, delta, static_cast<T*>(dq));
     if (const int rc = launch_status()) return rc;
     wattn_generic_dkv_kernel<T, NC><<<static_cast<unsigned>(keys), 32 * kGenWarps, smem_kv, st>>>(
         a, d, ds[0], ds[1], ds[2], lse, delta, static_cast<T*>(dk), static_cast<T*>(dv));
