@@ -33,3 +33,18 @@ def test_no_queries_in_c(device, dtype):
     assert _c("tops_window_attn_backward", _lib.dtype_code(dtype), B, 0, Nk, H, H, D, None, None, None, None, None, 3, 0, 0,
               1.0, None, None, None, None, None, None, dk, dv, ctypes.c_void_p(_lib.stream_ptr())) == _lib.OK
     assert not dk.any() and not dv.any()
+
+
+def test_decode_workspace_of_no_sequences():
+    """No division by the number of sequences, whatever the window."""
+    need = ctypes.c_int64(-1)
+    for window in (1, 4096, 9000, 2**40):
+        assert _c("tops_window_attn_decode_workspace_bytes", 0, 10000, 4, 2, 64, window, 0, ctypes.byref(need)) == _lib.OK
+        assert need.value == 0
+
+
+@gpu
+def test_decode_of_no_sequences(device):
+    k = torch.zeros(0, 10000, 2, 64, dtype=BF, device=device)
+    n = torch.zeros(0, dtype=torch.int32, device=device)
+    assert window_attn.decode(torch.zeros(0, 4, 64, dtype=BF, device=device), k, k, n, window=9000).shape == (0, 4, 64)

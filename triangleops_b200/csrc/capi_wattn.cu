@@ -121,7 +121,8 @@ extern "C" int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int
                                                        int64_t window, int64_t sinks, int64_t* bytes) {
   if (bytes == nullptr || window < 1 || sinks < 0) return TOPS_ERR_ARG;
   if (B < 0 || N < 1 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return TOPS_ERR_SHAPE;
-  *bytes = wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
+  // a plan divides the SMs among the sequences
+  *bytes = B == 0 ? 0 : wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
   return TOPS_OK;
 }
 
