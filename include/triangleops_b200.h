@@ -261,7 +261,8 @@ int tops_transition_forward(int dtype, int64_t M, int64_t C, const void* x, cons
 /* out = softmax(scale q k^T) v, where query i, at key position p = i + Nk - Nq, sees key j iff
  *   j <= p + right  and  (j >= p - left  or  j < sinks)  and  (mask == NULL or mask[b*Nk + j]).
  * q (B, Nq, Hq, D), k and v (B, Nk, Hkv, D), channels contiguous; strides[9] = {q: b, n, h;
- * k: b, n, h; v: b, n, h}. Query head h reads key head h / (Hq / Hkv). Nq <= Nk, D <= 256.
+ * k: b, n, h; v: b, n, h}. Query head h reads key head h / (Hq / Hkv). Nq <= Nk < 2^30, D <= 256,
+ * B and Hq D below 2^31, B Hq Nk below 2^33; beyond that TOPS_ERR_SHAPE.
  * out [B][Nq][Hq][D]; lse [B][Hq][Nq] (natural log of the row sums; NULL: not wanted). A query
  * that sees no key gets zeros and lse -inf. */
 int tops_window_attn_forward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,

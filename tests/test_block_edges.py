@@ -48,3 +48,19 @@ def test_decode_of_no_sequences(device):
     k = torch.zeros(0, 10000, 2, 64, dtype=BF, device=device)
     n = torch.zeros(0, dtype=torch.int32, device=device)
     assert window_attn.decode(torch.zeros(0, 4, 64, dtype=BF, device=device), k, k, n, window=9000).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,N,D", [(2**32, 1, 1, 1, 8), (2**32 + 1, 1, 1, 1, 8), (1, 2**32, 2**32, 1, 8), (1, 2**31, 1, 1, 8),
+                                          (2**31, 1, 1, 1, 64), (1, 2**26, 2**26, 1, 64)])
+def test_sizes_past_31_bits_are_refused(B, Hq, Hkv, N, D):
+    """The kernels count sequences, and the channels of a token, in 32 bits."""
+    t, st, need = torch.zeros(16, dtype=BF), [8] * 9, ctypes.c_int64(0)
+    assert _c("tops_window_attn_forward", _lib.BF16, B, N, N, Hq, Hkv, D, t, t, t, st, None, 3, 0, 0, 1.0, t, None,
+              None) == _lib.ERR_SHAPE
+    assert _c("tops_window_attn_backward", _lib.BF16, B, N, N, Hq, Hkv, D, t, t, t, st, None, 3, 0, 0, 1.0, t, [8] * 3, t, t,
+              t, t, t, t, None) == _lib.ERR_SHAPE
+    assert _c("tops_window_attn_backward_workspace_bytes", _lib.BF16, B, N, N, Hq, Hkv, D, 3, 0, 0,
+              ctypes.byref(need)) == _lib.ERR_SHAPE
+    assert _c("tops_window_attn_decode", _lib.BF16, B, N, Hq, Hkv, D, t, t, t, [8] * 8, t, 3, 0, 1.0, None, t,
+              None) == _lib.ERR_SHAPE
+    assert _c("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, 3, 0, ctypes.byref(need)) == _lib.ERR_SHAPE

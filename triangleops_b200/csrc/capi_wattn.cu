@@ -7,12 +7,19 @@
 
 namespace tops {
 
+// The sizes that the kernels can count: sequences, heads and the channels of a token in 31 bits, keys in 30
+// (a position plus a window fits 31).
+inline int wattn_sizes(int64_t B, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D) {
+  constexpr int64_t kInt = int64_t(1) << 31;
+  if (B < 0 || Nk < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return TOPS_ERR_SHAPE;
+  return B < kInt && Nk < kInt / 2 && Hq < kInt / D ? TOPS_OK : TOPS_ERR_SHAPE;
+}
+
 inline int wattn_args(WattnArgs& a, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
                       const void* q, const void* k, const void* v, const int64_t* st, const uint8_t* mask,
                       int64_t left, int64_t right, int64_t sinks, float scale) {
-  constexpr int64_t kMost = int64_t(1) << 30;
-  if (B < 0 || Nq < 0 || Nk < Nq || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return TOPS_ERR_SHAPE;
-  if (Nk >= kMost || B * Hq * Nk >= (int64_t(1) << 33)) return TOPS_ERR_SHAPE;
+  if (const int rc = wattn_sizes(B, Nk, Hq, Hkv, D)) return rc;
+  if (Nq < 0 || Nk < Nq || (Nk > 0 && B * Hq > ((int64_t(1) << 33) - 1) / Nk)) return TOPS_ERR_SHAPE;
   if (left < 0 || right < 0 || sinks < 0) return TOPS_ERR_ARG;
   if (B > 0 && Nq > 0 && (q == nullptr || k == nullptr || v == nullptr || st == nullptr)) return TOPS_ERR_ARG;
   a.B = static_cast<int>(B);
@@ -120,7 +127,8 @@ extern "C" int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, i
 extern "C" int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
                                                        int64_t window, int64_t sinks, int64_t* bytes) {
   if (bytes == nullptr || window < 1 || sinks < 0) return TOPS_ERR_ARG;
-  if (B < 0 || N < 1 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D > 256) return TOPS_ERR_SHAPE;
+  if (N < 1) return TOPS_ERR_SHAPE;
+  if (const int rc = wattn_sizes(B, N, Hq, Hkv, D)) return rc;
   // a plan divides the SMs among the sequences
   *bytes = B == 0 ? 0 : wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
   return TOPS_OK;
