@@ -289,6 +289,12 @@ int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t
                             int64_t window, int64_t sinks, float scale, void* workspace, void* out, void* stream);
 int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                                             int64_t sinks, int64_t* bytes);
+/* The keys and values k and v (B, Hkv, D) of one token for each sequence to place lengths[b] of the caches
+ * (B, N, Hkv, D). strides[4] = {k: b, h; v: b, h}, channels contiguous; cache_strides[8] = {k: b, n, h,
+ * channel; v: b, n, h, channel}. A sequence whose place is outside 0..N-1 writes nothing. */
+int tops_window_attn_store(int dtype, int64_t B, int64_t N, int64_t Hkv, int64_t D, const void* k, const void* v,
+                           const int64_t* strides, const int32_t* lengths, void* k_cache, void* v_cache,
+                           const int64_t* cache_strides, void* stream);
 
 /* u = post(y); r = u * sigmoid(gate); h = x + res_s * r; n = pre(h), over `rows` rows of C <= 8192
  * channels (row strides xs, ys, gs); layer != 0: LayerNorm, else RMS norm. has_post, has_pre: the

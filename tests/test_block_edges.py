@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import block_refs as ref
-from triangleops_b200 import _lib, window_attn
+from triangleops_b200 import _lib, local_block, window_attn
 
 gpu = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -64,3 +64,65 @@ def test_sizes_past_31_bits_are_refused(B, Hq, Hkv, N, D):
     assert _c("tops_window_attn_decode", _lib.BF16, B, N, Hq, Hkv, D, t, t, t, [8] * 8, t, 3, 0, 1.0, None, t,
               None) == _lib.ERR_SHAPE
     assert _c("tops_window_attn_decode_workspace_bytes", B, N, Hq, Hkv, D, 3, 0, ctypes.byref(need)) == _lib.ERR_SHAPE
+
+
+@gpu
+def test_step_without_room(device):
+    """Lengths that have no place in the caches: these sequences get NaN, the others what they would
+    get, and what the caches hold stays."""
+    g = torch.Generator().manual_seed(0)
+    pre = local_block.init(64, 4, 2, 16, 96, 2, sections=(4, 4), dtype=FP, device=device, generator=g)
+    B, N = 5, 6
+    s = torch.randn(B, 64, generator=g).to(device)
+    pos = torch.arange(B, dtype=torch.int32, device=device).expand(2, B)
+    full = local_block.caches(pre, B, N, dtype=FP, device=device)
+    for pair in full:
+        for c in pair:
+            c.copy_(torch.randn(c.shape, generator=g))
+    before = [[c.clone() for c in pair] for pair in full]
+    lengths = torch.tensor([N, 3, -1, N - 1, 2**31 - 1], dtype=torch.int32, device=device)
+    x, n = local_block.step(s, pre, pos, full, lengths, window=4, sinks=1)
+    fit = [1, 3]
+    some = [[c[fit] for c in pair] for pair in before]
+    x2, n2 = local_block.step(s[fit], pre, pos[:, fit], some, lengths[fit], window=4, sinks=1)
+    torch.testing.assert_close(x[fit], x2, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(n[fit], n2, rtol=1e-5, atol=1e-5)
+    for b in range(B):
+        assert (torch.isfinite if b in fit else torch.isnan)(torch.stack([x[b], n[b]])).all()
+    for pair, old in zip(full, before):
+        for c, o in zip(pair, old):
+            same = (c == o).all(-1).all(-1)  # (B, N)
+            for b in range(B):
+                assert same[b].tolist() == [b not in fit or t != lengths[b].item() for t in range(N)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_store(device, dtype):
+    """Any strides of what is stored and of the caches; lengths of either width."""
+    g = torch.Generator().manual_seed(1)
+    B, N, H, D = 4, 5, 3, 20
+    k, v = (torch.randn(B, H, D, generator=g).to(device, dtype) for _ in range(2))
+    lengths = torch.tensor([0, N - 1, N, 2], device=device)
+    want = [torch.zeros(B, N, H, D, dtype=dtype, device=device) for _ in range(2)]
+    for b, n in enumerate(lengths.tolist()):
+        if n < N:
+            want[0][b, n], want[1][b, n] = k[b], v[b]
+    both = torch.zeros(B, N, 2, H, D, dtype=dtype, device=device)
+    turned = [torch.zeros(B, D, H, N, dtype=dtype, device=device).permute(0, 3, 2, 1) for _ in range(2)]
+    split = torch.cat([k, v], 1)
+    for kc, vc, n in ((both[:, :, 0], both[:, :, 1], lengths), (*turned, lengths.int())):
+        window_attn.kernel.store(split[:, :H], v.transpose(1, 2).contiguous().transpose(1, 2), kc, vc, n)
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
+def test_store_refusals():
+    k, c, n = torch.zeros(2, 3, 8), torch.zeros(2, 4, 3, 8), torch.zeros(2, dtype=torch.int32)
+    store = window_attn.kernel.store
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        store(k, k, c, c, n)
+    for bad in ((k, k[:, :2], c, c, n), (k, k, c[:1], c, n), (k, k, c, c[:, :3], n), (k, k, c, c, n[:1]), (k[0], k[0], c, c, n)):
+        with pytest.raises(AssertionError):
+            store(*bad)
+    with pytest.raises(ValueError):
+        store(k, k, c.half(), c.half(), n)

@@ -232,6 +232,33 @@ PyObject* window_attn_decode(PyObject* const* a) {
   return give(out);
 }
 
+// (k, v, k_cache, v_cache, lengths) -> None
+PyObject* window_attn_store(PyObject* const* a) {
+  Tensor k = tensor(a[0]), v = tensor(a[1]), n = tensor(a[4]);
+  const Tensor kc = tensor(a[2]), vc = tensor(a[3]);
+  const int dt = dtype_code(k);
+  must(k.dim() == 3 && k.sizes() == v.sizes(), "k and v must be (B, Hkv, D)");
+  const int64_t B = k.size(0), H = k.size(1), D = k.size(2);
+  must(kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.size(0) == B && kc.size(2) == H && kc.size(3) == D,
+       "the caches must be (B, N, Hkv, D) like k and v");
+  must(n.dim() == 1 && n.size(0) == B, "lengths must be (B,)");
+  same_dtype(k, v, "k, v and the caches");
+  same_dtype(k, kc, "k, v and the caches");
+  same_dtype(k, vc, "k, v and the caches");
+  must(v.device() == k.device() && kc.device() == k.device() && vc.device() == k.device() && n.device() == k.device(),
+       "k, v, the caches and lengths must be on one device");
+  require_cuda(k);
+  const c10::cuda::CUDAGuard guard(k.device());
+  k = rows(k), v = rows(v), n = n.to(at::kInt).contiguous();
+  const int64_t st[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
+  int64_t ct[8];
+  for (int i = 0; i < 4; ++i) ct[i] = kc.stride(i), ct[4 + i] = vc.stride(i);
+  check(tops_window_attn_store(dt, B, kc.size(1), H, D, ptr(k), ptr(v), st, static_cast<const int32_t*>(ptr(n)),
+                               out_ptr(kc), out_ptr(vc), ct, stream_of(k)),
+        "tops_window_attn_store");
+  Py_RETURN_NONE;
+}
+
 // ---------------------------------------------------------------------------
 // gated norms
 // ---------------------------------------------------------------------------
@@ -443,8 +470,9 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define TOPS_METHOD(f, n) \
   { #f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(call<f, n>)), METH_FASTCALL, nullptr }
 PyMethodDef methods[] = {TOPS_METHOD(window_attn_forward, 9), TOPS_METHOD(window_attn_backward, 11),
-                         TOPS_METHOD(window_attn_decode, 7),  TOPS_METHOD(gated_norm_forward, 12),
-                         TOPS_METHOD(gated_norm_backward, 14), TOPS_METHOD(rotary, 7),
+                         TOPS_METHOD(window_attn_decode, 7),  TOPS_METHOD(window_attn_store, 5),
+                         TOPS_METHOD(gated_norm_forward, 12), TOPS_METHOD(gated_norm_backward, 14),
+                         TOPS_METHOD(rotary, 7),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bind", "Launchers of the token block's operators.", -1, methods};
 

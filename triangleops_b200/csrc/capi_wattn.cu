@@ -158,3 +158,27 @@ extern "C" int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t 
   }
   return by_io_type(dtype, [&](auto t) { return run_wattn_generic<decltype(t)>(a, out, nullptr, st); });
 }
+
+extern "C" int tops_window_attn_store(int dtype, int64_t B, int64_t N, int64_t Hkv, int64_t D, const void* k, const void* v,
+                                      const int64_t* strides, const int32_t* lengths, void* k_cache, void* v_cache,
+                                      const int64_t* cache_strides, void* stream) {
+  if (dtype != TOPS_BF16 && dtype != TOPS_F16 && dtype != TOPS_F32) return TOPS_ERR_DTYPE;
+  if (const int rc = wattn_sizes(B, N, Hkv, Hkv, D)) return rc;
+  if (B == 0 || N == 0) return TOPS_OK;
+  if (k == nullptr || v == nullptr || strides == nullptr || lengths == nullptr || k_cache == nullptr ||
+      v_cache == nullptr || cache_strides == nullptr)
+    return TOPS_ERR_ARG;
+  WattnStoreArgs a;
+  for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < 2; ++i) a.from[t][i] = strides[2 * t + i];
+    for (int i = 0; i < 4; ++i) a.to[t][i] = cache_strides[4 * t + i];
+  }
+  a.src[0] = k, a.src[1] = v, a.dst[0] = k_cache, a.dst[1] = v_cache, a.lengths = lengths;
+  a.N = static_cast<int>(N), a.H = static_cast<int>(Hkv), a.D = static_cast<int>(D);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == TOPS_F32)
+    wattn_store_kernel<uint32_t><<<static_cast<unsigned>(B), 256, 0, st>>>(a);
+  else
+    wattn_store_kernel<uint16_t><<<static_cast<unsigned>(B), 256, 0, st>>>(a);
+  return launch_status();
+}

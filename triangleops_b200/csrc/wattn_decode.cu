@@ -315,6 +315,27 @@ __global__ void __launch_bounds__(DT) wattn_decode_join_kernel(const WattnDecode
       E::from_f(y == 0.f ? 0.f : x / y);
 }
 
+// The key and value rows of one token a sequence to their place in the caches, W: the type's width. A
+// place that the caches do not have is not written.
+struct WattnStoreArgs {
+  int64_t from[2][2], to[2][4];  // strides of k and v (batch, head), of the caches (batch, token, head, channel)
+  const void* src[2];
+  void* dst[2];
+  const int* lengths;
+  int N, H, D;
+};
+template <typename W>
+__global__ void __launch_bounds__(256) wattn_store_kernel(const WattnStoreArgs a) {
+  const int64_t b = blockIdx.x;
+  const int at = a.lengths[b], row = a.H * a.D;
+  if (at < 0 || at >= a.N) return;
+  for (int i = threadIdx.x; i < row; i += 256)
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      static_cast<W*>(a.dst[t])[b * a.to[t][0] + at * a.to[t][1] + i / a.D * a.to[t][2] + i % a.D * a.to[t][3]] =
+          static_cast<const W*>(a.src[t])[b * a.from[t][0] + i / a.D * a.from[t][1] + i % a.D];
+}
+
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------

@@ -105,17 +105,19 @@ def caches(pre, B, N, *, dtype, device=None):
 def step(s, pre, positions, cache, lengths, *, window, sinks=0, eps=1e-5):
     """One token for each sequence: s (B, C), positions (axes, B); its keys and values go to
     place ``lengths[b]`` (B,) int32 of the caches, which then hold ``lengths + 1`` tokens.
-    ``window`` is a number of keys. Returns (s, n), each (B, C)."""
+    ``window`` is a number of keys. Returns (s, n), each (B, C). A sequence whose place the caches
+    do not have (they are full, or the length is negative) leaves them as they are and gets NaN."""
     x = s.unsqueeze(1)
     n = _first_norm(x, pre, eps)
-    row, now = torch.arange(s.shape[0], device=s.device), lengths + 1
+    N = min((kc.shape[1] for kc, _ in cache), default=2**31 - 1)
+    out = ((lengths < 0) | (lengths >= N)).unsqueeze(-1)
+    now = lengths + 1
     for b, (kc, vc) in zip(pre["blocks"], cache):
         q, k, v, g = _project(n, b, pre)
         q, k = _rot.rotary(q, k, positions.unsqueeze(-1), **pre["rotary"])
-        kc[row, lengths.long()] = k[:, 0]
-        vc[row, lengths.long()] = v[:, 0]
+        _wa.kernel.store(k[:, 0], v[:, 0], kc, vc, lengths)
         o = _wa.decode(q[:, 0], kc, vc, now, window=window, sinks=sinks)
         x, n = _gn.gated_norm(x, F.linear(o.flatten(-2), b["w_o"]).unsqueeze(1), g, kind=pre["kind"], eps=eps,
                               **b["attn"])
         x, n = _transition(x, n, b, pre, eps)
-    return x[:, 0], n[:, 0]
+    return x[:, 0].masked_fill(out, float("nan")), n[:, 0].masked_fill(out, float("nan"))

@@ -58,3 +58,9 @@ def decode(q, k_cache, v_cache, lengths, *, window, sinks=0, scale=None):
     if not isinstance(window, int):
         raise ValueError(f"window must be a number of keys, at least 1, got {window}")
     return _lib.bind().window_attn_decode(q, k_cache, v_cache, lengths, window, sinks, scale)
+
+
+def store(k, v, k_cache, v_cache, lengths):
+    """The keys and values (B, Hkv, D) of one token for each sequence to place ``lengths[b]`` of the
+    caches. A sequence whose place the caches do not have (below 0, or N and beyond) writes nothing."""
+    _lib.bind().window_attn_store(k, v, k_cache, v_cache, lengths)
