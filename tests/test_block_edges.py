@@ -126,3 +126,19 @@ def test_store_refusals():
             store(*bad)
     with pytest.raises(ValueError):
         store(k, k, c.half(), c.half(), n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("B,N,H,window,sinks", [(65537, 2, 1, 2, 0), (65540, 3, 2, 1, 1), (8200, 140, 8, 2, 1)])
+def test_gradients_of_many_sequences(device, dtype, B, N, H, window, sinks):
+    """More sequences than a grid's second and third dimensions count, with and without sinks' late queries."""
+    g = torch.Generator(device=device).manual_seed(N)
+    q, k, v, d = (torch.randn(B, N, H, 8, device=device, generator=g).to(dtype) for _ in range(4))
+    kw = dict(window=window, sinks=sinks)
+    out, lse = window_attn.forward(q, k, v, **kw)
+    got = dict(zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, **kw)), out=out)
+    rows = torch.tensor([0, 1, B // 2, B - 2, B - 1], device=device)
+    want = ref.attention(q[rows], k[rows], v[rows], window, sinks, dout=d[rows])
+    for name, t in got.items():
+        ref.assert_within(t[rows], *want[name], f"{name} {dtype} {(B, N, H)}")

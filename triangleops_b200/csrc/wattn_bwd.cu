@@ -27,6 +27,7 @@
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
 // end, has -lse2 = -inf, so that its P is 0.
+#include <algorithm>
 #include "sm100.cuh"
 #include "wattn.h"
 
@@ -483,9 +484,11 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
                                                           float* __restrict__ lse2, float* __restrict__ delta) {
   using E = Elem<T>;
   pdl_trigger();
-  const int i = static_cast<int>((blockIdx.x * 256u + threadIdx.x) >> 3), part = threadIdx.x & 7;
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
+  // blocks of 32 queries, then heads, then sequences: all in x, whose range the tiles' grid shares
+  const unsigned blocks = nqp / 32;
+  const int i = static_cast<int>(blockIdx.x % blocks * 32 + (threadIdx.x >> 3)), part = threadIdx.x & 7;
+  const int64_t bh = blockIdx.x / blocks;
+  const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
   float x = 0.f, v = -INFINITY;
   if (i < a.Nq) {
     const T* d = dout + b * s0 + i * s1 + h * s2;
@@ -510,7 +513,7 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
   }
 #pragma unroll
   for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if (part == 0 && i < nqp) {
+  if (part == 0) {
     lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : -v * kLog2e;
     delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
   }
@@ -528,9 +531,10 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) 
   using W = WattnParts<DT>;
   __shared__ float sum[W::SHARES][W::ROWS * W::PER][9];
   const int at = threadIdx.x % (W::PER * W::ROWS), share = threadIdx.x / (W::PER * W::ROWS);
-  const int row = blockIdx.x * W::ROWS + at / W::PER, col = at % W::PER * 8;
-  const int which = blockIdx.y & 1, kb = blockIdx.y >> 1;
-  const int64_t bh = blockIdx.z;
+  const unsigned pairs = (a.keep + W::ROWS - 1) / W::ROWS, unit = blockIdx.x / pairs;
+  const int row = blockIdx.x % pairs * W::ROWS + at / W::PER, col = at % W::PER * 8;
+  const int which = unit & 1, kb = (unit >> 1) % a.nsb;
+  const int64_t bh = (unit >> 1) / a.nsb;
   const int key = kb * 128 + row;
   const bool live = row < a.keep && key < a.sinks && col < a.D;
   const int n = live ? 1 + a.group * a.nx : 0;
@@ -595,7 +599,6 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
   bind_context();
   const WattnBwdPlan p = wattn_bwd_plan(a, a.Nq);
   float *lse2 = ws, *delta = ws + p.stats;
-  if (a.Hq > 65535 || a.B > 65535) return TOPS_ERR_SHAPE;
   CUtensorMap mq, mk, mv, md;
   if (!wattn_map(&mq, dtype, a.q, a.qs, a.B, a.Nq, a.Hq, a.D, 64) ||
       !wattn_map(&md, dtype, dout, ds, a.B, a.Nq, a.Hq, a.D, 64) ||
@@ -612,21 +615,19 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
   f.tiles = (a.Nk + 127) / 128, f.q_tiles = (a.Nq + 127) / 128;
   const int64_t own = heads * f.tiles, kv = own + heads * p.nsb * f.group * p.nx;
   const int64_t grid = kv + static_cast<int64_t>(f.q_tiles) * a.Hq * a.B;
-  if (grid >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
-  if (p.nsb > 0 && (heads > 65535 || p.nsb > 32767)) return TOPS_ERR_SHAPE;
+  const int64_t stats = static_cast<int64_t>(a.B) * a.Hq * (p.nqp / 32);
+  constexpr int ROWS = WattnParts<DT>::ROWS;
+  const int64_t parts = heads * 2 * p.nsb * ((p.keep + ROWS - 1) / ROWS);
+  if (std::max(std::max(grid, stats), parts) >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   f.own = static_cast<int>(own), f.kv_blocks = static_cast<int>(kv), f.dq = dq, f.dk = dk, f.dv = dv;
-  wattn_stats_kernel<T, DT><<<dim3((p.nqp + 31) / 32, a.Hq, a.B), 256, 0, st>>>(
+  wattn_stats_kernel<T, DT><<<static_cast<unsigned>(stats), 256, 0, st>>>(
       a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
   const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
   auto kern = wattn_backward_kernel<T, DT>;
   static std::atomic<uint64_t> done{0};
   set_smem_once(kern, smem, done);
   launch_pdl(kern, static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st, mq, md, mk, mv, f);
-  if (f.nsb > 0) {
-    constexpr int ROWS = WattnParts<DT>::ROWS;
-    launch_pdl(wattn_parts_kernel<T, DT>, dim3((p.keep + ROWS - 1) / ROWS, 2 * f.nsb, static_cast<unsigned>(heads)), 256,
-               0, st, f);
-  }
+  if (f.nsb > 0) launch_pdl(wattn_parts_kernel<T, DT>, static_cast<unsigned>(parts), 256, 0, st, f);
   return launch_status();
 }
 
