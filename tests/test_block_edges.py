@@ -142,3 +142,29 @@ def test_gradients_of_many_sequences(device, dtype, B, N, H, window, sinks):
     want = ref.attention(q[rows], k[rows], v[rows], window, sinks, dout=d[rows])
     for name, t in got.items():
         ref.assert_within(t[rows], *want[name], f"{name} {dtype} {(B, N, H)}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("low", [-16.0, -17.0, -20.0])
+def test_probabilities_far_below_the_largest(device, dtype, low):
+    """A first key that takes nearly all and holds zeros, and some thousand keys e^-16 to e^-20 below
+    it that make the result: they count, although f16 has nothing below 2^-24. (Held at 2^11 times its
+    size, a probability is off by 2^-36 of the largest at most; one token's at 2^15.)"""
+    N, D = 2048, 64
+    g = torch.Generator().manual_seed(7)
+    q = torch.ones(1, N, 1, D).to(device, dtype)
+    k = torch.full((1, N, 1, D), low / 64).to(device, dtype)  # scores of `low`, exact in either type
+    k[:, 0] = 0.0
+    v = (1 + torch.rand(1, N, 1, D, generator=g)).to(device, dtype)
+    v[:, 0] = 0.0
+    want = ref.attention(q, k, v, N, 1, scale=1.0)
+    value, bound = want["out"]
+    sums = v.double().cumsum(1) if dtype == HF else torch.zeros_like(value)
+    out, lse = window_attn.forward(q, k, v, window=N, sinks=1, scale=1.0)
+    ref.assert_within(out, value, bound + 2.0**-36 * sums, "out")
+    torch.testing.assert_close(lse.double(), want["lse"][0], rtol=1e-5, atol=1e-5)
+    # the last query alone, through the one-token form
+    n = torch.tensor([N], dtype=torch.int32, device=device)
+    one = window_attn.decode(q[:, -1].contiguous(), k, v, n, window=N, sinks=1, scale=1.0)
+    ref.assert_within(one, value[:, -1], (bound + 2.0**-40 * sums)[:, -1], "one token")

@@ -91,6 +91,8 @@ template <typename T, int DT, int NW>
 __global__ void __launch_bounds__(32 * NW, NW == 2 ? 4 : 1) wattn_decode_kernel(const WattnDecodeArgs a) {
   using E = Elem<T>;
   constexpr int NS = DT / 32, NU = DT / 64;
+  // f16 ends at 2^-24: p, at most 1, is held at 2^15 times its size, the sums with it
+  constexpr float kLift = E::kFmt == 0 ? 15.f : 0.f;
   extern __shared__ uint8_t smem_raw[];
   auto& sm = *reinterpret_cast<WattnDecodeSmem<DT, NW>*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane >> 2, t4 = lane & 3;
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(32 * NW, NW == 2 ? 4 : 1) wattn_decode_kernel(
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float base = m[r] == -INFINITY ? 0.f : m[r];
+        const float base = m[r] == -INFINITY ? 0.f : m[r] - kLift;
         const float p0 = ex2_approx(s[nt][2 * r] - base), p1 = ex2_approx(s[nt][2 * r + 1] - base);
         l[r] += p0 + p1;
         pa[2 * nt + r] = E::pack2(p0, p1);
