@@ -168,3 +168,53 @@ def test_probabilities_far_below_the_largest(device, dtype, low):
     n = torch.tensor([N], dtype=torch.int32, device=device)
     one = window_attn.decode(q[:, -1].contiguous(), k, v, n, window=N, sinks=1, scale=1.0)
     ref.assert_within(one, value[:, -1], (bound + 2.0**-40 * sums)[:, -1], "one token")
+
+
+def _norm_error(got, value):
+    return (torch.linalg.vector_norm(got.double() - value) / torch.linalg.vector_norm(value)).item()
+
+
+@gpu
+@pytest.mark.parametrize("N,Nq,Hq,Hkv,D,window,sinks,masked", [(2048, 2048, 2, 1, 64, 512, 4, False),
+                                                              (1500, 700, 2, 2, 128, (200, 20), 0, True),
+                                                              (1000, 1000, 4, 1, 32, (40, 0), 140, True)])
+@pytest.mark.parametrize("dout,v_sd", [(1e-6, 1.0), (1e-4, 1.0), (1e-3, 1.0), (1.0, 1.0), (500.0, 30.0), (1.0, 1e-4)])
+def test_f16_gradients_of_any_size(device, dout, v_sd, N, Nq, Hq, Hkv, D, window, sinks, masked):
+    """Gradients far below and above 1: f16 products keep their digits. The 2-norm may be off by the
+    store and by one 16-bit factor of a product (2^-11 of the value each), and by half of f16's
+    smallest step for each element. What masked keys and queries that see nothing hold sizes nothing."""
+    g = torch.Generator().manual_seed(D)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    q, k, v = r(1, Nq, Hq, D).to(device, HF), r(1, N, Hkv, D).to(device, HF), (r(1, N, Hkv, D) * v_sd).to(device, HF)
+    d = (r(1, Nq, Hq, D) * dout).to(device, HF)
+    mask = None
+    if masked:
+        mask = torch.rand(1, N, generator=g).to(device) < 0.8
+        mask[:, -60:] = False
+        v = v.masked_fill(~mask[..., None, None], 60000.0)
+    want = ref.attention(q, k, v, window, sinks, mask, dout=d)
+    kw = dict(window=window, sinks=sinks, mask=mask)
+    out, lse = window_attn.forward(q, k, v, **kw)
+    for name, got in zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, **kw)):
+        value = want[name][0]
+        fits = value.abs() < 65520.0  # what rounds to infinity is infinite
+        assert torch.equal(torch.isfinite(got), fits), name
+        got, value = got[fits], value[fits]
+        off = torch.linalg.vector_norm(got.double() - value).item()
+        size = torch.linalg.vector_norm(value).item()
+        assert off <= 2.0**-10 * size + 2.0**-25 * value.numel() ** 0.5, (name, off / size)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_gradients_of_q_and_k_lose_only_their_own_rounding(device, dtype):
+    """dS enters its products with twice the type's digits: dQ and dK are no farther from the 64-bit
+    values than these rounded (one more rounding of that size would add in squares: 1.4 times)."""
+    g = torch.Generator().manual_seed(3)
+    q, k, v, d = (torch.randn(2, 1024, h, 64, generator=g).to(device, dtype) for h in (4, 2, 2, 4))
+    want = ref.attention(q, k, v, 256, 4, dout=d)
+    out, lse = window_attn.forward(q, k, v, window=256, sinks=4)
+    dq, dk, _ = window_attn.backward(d, q, k, v, out, lse, window=256, sinks=4)
+    for name, got in (("dq", dq), ("dk", dk)):
+        value = want[name][0]
+        assert _norm_error(got, value) <= 1.2 * _norm_error(value.to(dtype), value), name

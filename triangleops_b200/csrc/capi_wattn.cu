@@ -120,7 +120,7 @@ extern "C" int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, i
     return rc;
   if (Nq < 0 || Nq > Nk) return TOPS_ERR_SHAPE;
   const WattnBwdPlan p = wattn_bwd_plan(a, Nq);
-  *bytes = (2 * p.stats + p.part) * 4;  // (the CUDA-core path needs less)
+  *bytes = (2 * p.stats + 4 + p.part) * 4;  // (the CUDA-core path needs less)
   return TOPS_OK;
 }
 

@@ -24,6 +24,12 @@
 // they fill the SMs that the last round of tiles leaves idle); their fp32 sums, and the tile's
 // own for these rows, are added in order by a last kernel.
 //
+// f16 has nothing below 2^-24 and ends at 65504, while dS is of the gradients' size. So in f16 both are held
+// at a power of two of their size: P at 2^14 times, which its exponent takes along, and dS at 2^14 / 2^e
+// times with 2^e above the largest |dP - delta| that there can be, 2 max |dO_i| max |v_j| over the queries
+// that see a key and the keys that a query may see; the statistics' kernel finds both. The results'
+// factors take the powers out again. bf16 has the range of the sums.
+//
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
 // end, has -lse2 = -inf, so that its P is 0.
@@ -45,6 +51,7 @@ struct WattnBwdArgs {
   const uint8_t* mask;
   float c, scale;
   const float *lse2, *delta;  // [B][Hq][nqp], negated
+  const unsigned* top;        // f16: the largest |dO_i|^2 and |v_j|^2, as bits
   void *dq, *dk, *dv;
   float* part;                // [B][Hkv][nsb][1 + group nx][2][keep][DT]
 };
@@ -72,6 +79,30 @@ struct WattnBwdSmem {
   uint32_t tmem_base;
   int abort;
 };
+
+// f16: P is held at 2^kWattnLift times its size (in the statistics' -lse2)
+constexpr float kWattnLift = 14.f;
+template <typename T>
+__device__ __forceinline__ float wattn_lift() {
+  return Elem<T>::kFmt == 0 ? kWattnLift : 0.f;
+}
+// What dS is multiplied with (f16: P is held at 2^14 times its size; |dP - delta| times `down` is below 1),
+// and the factors of dV and, before the scale, of dQ and dK that undo it.
+struct WattnScales {
+  float down = 1.f, dv = 1.f, ds = 1.f;
+};
+template <typename T>
+__device__ __forceinline__ WattnScales wattn_scales(const unsigned* top) {
+  WattnScales s;
+  if constexpr (Elem<T>::kFmt == 0) {
+    const float most = 2.f * sqrtf(__uint_as_float(top[0])) * sqrtf(__uint_as_float(top[1]));
+    const int e = most > 0.f ? ilogbf(most) + 1 : 0;
+    s.down = ldexpf(1.f, -e);
+    s.dv = ldexpf(1.f, -static_cast<int>(kWattnLift));
+    s.ds = ldexpf(s.dv, e);
+  }
+  return s;
+}
 
 // The walk of one block: which tiles stream by.
 template <bool KV>
@@ -287,6 +318,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
       delta = a.delta[q];
     }
     const f2 c2 = f2_both(a.c);
+    const WattnScales scales = wattn_scales<T>(a.top);
     bool ok = true;
     int next = walk.total > 0 ? walk.row(0) : 0;
     for (int it = 0; it < walk.total; ++it) {
@@ -367,8 +399,10 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
       for (int i = 0; i < 16; i += 2) {
         ulonglong2 n = make_ulonglong2(f2_both(delta), f2_both(delta));
         if constexpr (KV) n = s_del[i / 2];
-        unpair(f2_mul(f2_add(pair(y, i), n.x), pair(x, i)), y, i);
-        unpair(f2_mul(f2_add(pair(y, i + 1), n.y), pair(x, i + 1)), y, i + 1);
+        f2 d0 = f2_add(pair(y, i), n.x), d1 = f2_add(pair(y, i + 1), n.y);
+        if constexpr (E::kFmt == 0) d0 = f2_mul(d0, f2_both(scales.down)), d1 = f2_mul(d1, f2_both(scales.down));
+        unpair(f2_mul(d0, pair(x, i)), y, i);
+        unpair(f2_mul(d1, pair(x, i + 1)), y, i + 1);
       }
       if (edge) {  // (what an unseen pair's product holds may be NaN)
 #pragma unroll
@@ -411,7 +445,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
     if (walk.total > 0 && (!ok || !mbar_wait(&sm.acc_done, 0, abort, 527))) ok = false;
     if (ok) {
       tc_fence_after();
-      const float f = KV && g == 0 ? 1.f : a.scale;
+      const float f = KV && g == 0 ? scales.dv : scales.ds * a.scale;
       const bool zero = walk.total == 0;
       constexpr int COLS = KV ? DT : DT / 2;
       const int col0 = KV ? 0 : g * COLS;
@@ -475,47 +509,89 @@ __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
     wattn_backward_block<T, DT, false>(map_q, map_d, map_k, map_v, a);
 }
 
-// -delta, delta = sum_d dO O, and -lse2 = -lse log2(e) per query, in rows of nqp: queries past Nq, and
-// those that see nothing, get -inf and 0. Eight threads a query, 16-byte loads.
+// -delta, delta = sum_d dO O, and -lse2 = -lse log2(e) (f16: + 14) per query, in rows of nqp: queries past
+// Nq, and those that see nothing, get -inf and 0. f16: the largest |dO|^2 of those that see something, and
+// (blocks behind the queries') the largest |v|^2 of the keys that the mask keeps, of `keys` from `key0` on
+// and of the sinks before them. Eight threads a row, 16-byte loads.
 template <typename T, int DT>
 __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* __restrict__ dout, int64_t s0,
                                                           int64_t s1, int64_t s2, const T* __restrict__ out,
-                                                          const float* __restrict__ lse, int nqp,
-                                                          float* __restrict__ lse2, float* __restrict__ delta) {
+                                                          const float* __restrict__ lse, int nqp, unsigned q_blocks,
+                                                          int key0, int keys, float* __restrict__ lse2,
+                                                          float* __restrict__ delta, unsigned* __restrict__ top) {
   using E = Elem<T>;
+  constexpr bool TOP = E::kFmt == 0;
   pdl_trigger();
-  // blocks of 32 queries, then heads, then sequences: all in x, whose range the tiles' grid shares
-  const unsigned blocks = nqp / 32;
-  const int i = static_cast<int>(blockIdx.x % blocks * 32 + (threadIdx.x >> 3)), part = threadIdx.x & 7;
-  const int64_t bh = blockIdx.x / blocks;
-  const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
-  float x = 0.f, v = -INFINITY;
-  if (i < a.Nq) {
-    const T* d = dout + b * s0 + i * s1 + h * s2;
-    const T* o = out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D;
-    uint4 u[DT / 64], w[DT / 64];
+  const int part = threadIdx.x & 7, in = threadIdx.x >> 3;
+  auto load = [&](const T* p, uint4* u) {
 #pragma unroll
     for (int k = 0; k < DT / 64; ++k) {
       const int c = part * 8 + 64 * k;
-      u[k] = w[k] = make_uint4(0, 0, 0, 0);
-      if (c < a.D) {
-        u[k] = *reinterpret_cast<const uint4*>(d + c);
-        w[k] = *reinterpret_cast<const uint4*>(o + c);
-      }
+      u[k] = make_uint4(0, 0, 0, 0);
+      if (c < a.D) u[k] = *reinterpret_cast<const uint4*>(p + c);
     }
-    if (part == 0) v = lse[bh * a.Nq + i];
+  };
+  auto dot = [&](const uint4* u, const uint4* w) {
+    float x = 0.f;
 #pragma unroll
     for (int k = 0; k < DT / 64; ++k) {
       const uint32_t *p = &u[k].x, *q = &w[k].x;
 #pragma unroll
       for (int e = 0; e < 4; ++e) x = fmaf(E::lo(p[e]), E::lo(q[e]), fmaf(E::hi(p[e]), E::hi(q[e]), x));
     }
-  }
 #pragma unroll
-  for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  if (part == 0) {
-    lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : -v * kLog2e;
-    delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
+    for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+  };
+  uint4 u[DT / 64], w[DT / 64];
+  float size = 0.f;  // |dO|^2 or |v|^2 of the row
+  // blocks of 32 queries, then heads, then sequences: all in x, whose range the tiles' grid shares
+  if (!TOP || blockIdx.x < q_blocks) {
+    const unsigned blocks = nqp / 32;
+    const int i = static_cast<int>(blockIdx.x % blocks * 32 + in);
+    const int64_t bh = blockIdx.x / blocks;
+    const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
+    float x = 0.f, v = -INFINITY;
+    if (i < a.Nq) {
+      load(dout + b * s0 + i * s1 + h * s2, u);
+      load(out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D, w);
+      v = lse[bh * a.Nq + i];
+    } else {
+#pragma unroll
+      for (int k = 0; k < DT / 64; ++k) u[k] = w[k] = make_uint4(0, 0, 0, 0);
+    }
+    x = dot(u, w);
+    if (TOP) size = dot(u, u);
+    if (v == -INFINITY) size = 0.f;
+    if (part == 0) {
+      lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : wattn_lift<T>() - v * kLog2e;
+      delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
+    }
+  } else {
+    const unsigned blocks = (keys + 31) / 32, unit = blockIdx.x - q_blocks;
+    const int i = static_cast<int>(unit % blocks * 32 + in), sinks = min(a.sinks, key0);
+    const int64_t bh = unit / blocks;
+    const int h = static_cast<int>(bh % a.Hkv), b = static_cast<int>(bh / a.Hkv);
+    const int j = i < sinks ? i : key0 + i - sinks;
+    const bool there = i < keys && (a.mask == nullptr || a.mask[static_cast<int64_t>(b) * a.Nk + j] != 0);
+#pragma unroll
+    for (int k = 0; k < DT / 64; ++k) u[k] = make_uint4(0, 0, 0, 0);
+    if (there) load(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + h * a.vs[2], u);
+    size = dot(u, u);
+  }
+  if constexpr (TOP) {
+    // what is not finite makes the results so wherever it goes, and says nothing of the others' size
+    unsigned bits = size < INFINITY ? __float_as_uint(size) : 0u;
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    __shared__ unsigned most[8];
+    if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = bits;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int i = 1; i < 8; ++i) bits = max(bits, most[i]);
+      unsigned* t = top + (blockIdx.x < q_blocks ? 0 : 1);
+      if (bits > *reinterpret_cast<volatile unsigned*>(t)) atomicMax(t, bits);  // (a maximum has no order)
+    }
   }
 }
 
@@ -556,7 +632,8 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) 
   for (int s = 1; s < W::SHARES; ++s)
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] += sum[s][at][k];
-  const float f = which == 0 ? 1.f : a.scale;
+  const WattnScales scales = wattn_scales<T>(a.top);
+  const float f = which == 0 ? scales.dv : scales.ds * a.scale;
   const int64_t b = bh / a.Hkv, hk = bh % a.Hkv;
   T* dst = static_cast<T*>(which == 0 ? a.dv : a.dk) + ((b * a.Nk + key) * a.Hkv + hk) * a.D + col;
   *reinterpret_cast<uint4*>(dst) = make_uint4(E::pack2(v[0] * f, v[1] * f), E::pack2(v[2] * f, v[3] * f),
@@ -568,7 +645,7 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) 
 // ---------------------------------------------------------------------------
 struct WattnBwdPlan {
   int nqp, nsb, nx, per, keep;
-  int64_t stats, part;  // elements of each of lse2 and delta; of the sinks' parts
+  int64_t stats, part;  // elements of each of lse2 and delta (and 4 for the largest sizes); of the sinks' parts
 };
 
 inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
@@ -610,18 +687,26 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
   f.left = a.left, f.right = a.right, f.sinks = a.sinks;
   f.nsb = p.nsb, f.nx = p.nx, f.per = p.per, f.keep = p.keep, f.nqp = p.nqp, f.mask = a.mask;
   f.c = a.scale * kLog2e, f.scale = a.scale, f.lse2 = lse2, f.delta = delta;
-  f.part = ws + 2 * p.stats;
+  f.part = ws + 2 * p.stats + 4;
   const int64_t heads = static_cast<int64_t>(a.B) * a.Hkv;
   f.tiles = (a.Nk + 127) / 128, f.q_tiles = (a.Nq + 127) / 128;
   const int64_t own = heads * f.tiles, kv = own + heads * p.nsb * f.group * p.nx;
   const int64_t grid = kv + static_cast<int64_t>(f.q_tiles) * a.Hq * a.B;
-  const int64_t stats = static_cast<int64_t>(a.B) * a.Hq * (p.nqp / 32);
+  // f16: the keys from the first query's window on and the sinks before them, for their largest value
+  unsigned* top = reinterpret_cast<unsigned*>(ws + 2 * p.stats);
+  const bool f16 = dtype == TOPS_F16;
+  const int key0 = std::max(0, a.Nk - a.Nq - a.left), keys = a.Nk - key0 + std::min(a.sinks, key0);
+  const int64_t q_blocks = static_cast<int64_t>(a.B) * a.Hq * (p.nqp / 32);
+  const int64_t stats = q_blocks + (f16 ? heads * ((keys + 31) / 32) : 0);
   constexpr int ROWS = WattnParts<DT>::ROWS;
   const int64_t parts = heads * 2 * p.nsb * ((p.keep + ROWS - 1) / ROWS);
   if (std::max(std::max(grid, stats), parts) >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   f.own = static_cast<int>(own), f.kv_blocks = static_cast<int>(kv), f.dq = dq, f.dk = dk, f.dv = dv;
+  if (f16 && cudaMemsetAsync(top, 0, 8, st) != cudaSuccess) return TOPS_ERR_CUDA;
+  f.top = top;
   wattn_stats_kernel<T, DT><<<static_cast<unsigned>(stats), 256, 0, st>>>(
-      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, lse2, delta);
+      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp,
+      static_cast<unsigned>(q_blocks), key0, keys, lse2, delta, top);
   const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
   auto kern = wattn_backward_kernel<T, DT>;
   static std::atomic<uint64_t> done{0};
