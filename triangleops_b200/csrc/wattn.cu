@@ -16,7 +16,7 @@
 // softmax: a thread owns a query row (a TMEM lane), so row maximum and sum need no exchange. S is a
 // fp32 TMEM tile, P takes its place rounded to the IO dtype (the product's operand type; its sum is
 // taken before the rounding), O accumulates in TMEM and is rescaled only when the maximum has grown
-// by 2^8 (f16: 2^4). S has two buffers: q k^T of the next block runs under the softmax of this one. Two CTAs
+// by 2^8 (f16: 2^7). S has two buffers: q k^T of the next block runs under the softmax of this one. Two CTAs
 // share an SM and its 512 TMEM columns (S 2 x 64, O up to 128 each). CTAs are persistent: the loads
 // and S of the next tile run under the end of the present one (8192 queries, 16 heads, window 1024:
 // 87.5 us with a CTA a tile, 83.6 so).
@@ -254,13 +254,14 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
     const int wq = warp & 3;
     const int row = wq * 32 + lane;  // TMEM lane = query row of the tile
     const uint32_t lane_addr = tbase + (static_cast<uint32_t>(wq * 32) << 16);
-    // f16 ends at 2^-24: P is held at 2^11 times its size, the sum with it, and the maximum may lag by 2^4
-    // there: a key keeps all its digits down to 2^-25 of the largest and counts down to 2^-36 (without
-    // it the many small probabilities of a window, beside a sink that takes most, are zeros). bf16 has
-    // the range and takes the longer lag.
+    // f16 ends at 2^-24: P is held at 2^8 times its size, the sum with it, and the maximum may lag by 2^7
+    // there: a key keeps all its digits down to 2^-22 of the largest and counts down to 2^-33 (without
+    // it the many small probabilities of a window, beside a sink that takes most, are zeros). Lags of 7,
+    // 6 and 4 that leave more room take 54.2, 55.5 and 68 us for 2 x 4096 queries, 16 heads of 128,
+    // window 512 (8 without the factor: 54.2). bf16 has the range.
     constexpr bool F16 = E::kFmt == 0;
-    constexpr float kLift = F16 ? 11.f : 0.f;
-    const float c = a.c, grow = (F16 ? 4.f : 8.f) / c;
+    constexpr float kLift = F16 ? 8.f : 0.f;
+    const float c = a.c, grow = (F16 ? 7.f : 8.f) / c;
     bool ok = true;
     for (int u = blockIdx.x; ok && u < a.units; u += gridDim.x, next()) {
     const WattnBlocks<6> blk = blocks(tile);
