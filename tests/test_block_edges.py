@@ -218,3 +218,28 @@ def test_gradients_of_q_and_k_lose_only_their_own_rounding(device, dtype):
     for name, got in (("dq", dq), ("dk", dk)):
         value = want[name][0]
         assert _norm_error(got, value) <= 1.2 * _norm_error(value.to(dtype), value), name
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("N,D,sinks,window", [(200, 64, 0, (30, 5)), (700, 128, 3, (100, 0)), (130, 32, 1, (8, 8))])
+def test_what_a_query_that_sees_nothing_holds(device, dtype, N, D, sinks, window):
+    """NaN and infinity in q and in the gradient of queries whose keys are all masked reach nothing."""
+    g = torch.Generator().manual_seed(N)
+    q, k, v, d = (torch.randn(2, N, h, D, generator=g).to(device, dtype) for h in (4, 2, 2, 4))
+    mask = torch.ones(2, N, dtype=torch.bool)
+    mask[0, :sinks] = mask[1, :sinks] = False  # (a kept sink is seen by all)
+    mask[0, N // 2:] = False
+    mask[1, 40:40 + window[0] + window[1] + 9] = False
+    mask = mask.to(device)
+    see = ref.visible(N, N, *window, sinks, mask, device)[:, 0].any(-1)  # (B, N)
+    assert (~see).any(1).all()
+    want = ref.attention(q, k, v, window, sinks, mask, dout=d)
+    kw = dict(window=window, sinks=sinks, mask=mask)
+    gone = ~see[..., None, None]
+    q, d = q.masked_fill(gone, float("nan")), d.masked_fill(gone, float("nan"))
+    d[..., 1::2] = d[..., 1::2].masked_fill(gone, float("inf"))
+    out, lse = window_attn.forward(q, k, v, **kw)
+    ref.assert_within(out, *want["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, **kw)):
+        ref.assert_within(got, *want[name], f"{name} {dtype}")

@@ -32,7 +32,7 @@
 //
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
-// end, has -lse2 = -inf, so that its P is 0.
+// end, has -lse2 = -inf, so that its P is 0; (KV) its rows of the q and dO tiles are zeroed likewise.
 #include <algorithm>
 #include "sm100.cuh"
 #include "wattn.h"
@@ -383,6 +383,24 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
 #pragma unroll
         for (int i = 0; i < 32; ++i)
           if (!(see >> i & 1)) x[i] = 0u;
+      }
+      if (KV && a.mask && wq == 0) {
+        // T1 and T2 of this tile are done: rows of queries that see nothing may be zeroed for P^T dO and
+        // dS^T q, so that no NaN there meets a P of 0
+        const bool none = sm.st[r][0][32 * g + lane] == -INFINITY;
+        if (__any_sync(0xffffffffu, none)) {
+          if (none) {
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int to = u * 64 * 128 + (32 * g + lane) * 128;
+                reinterpret_cast<uint4*>(sm.b1[r] + to)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(sm.b2[r] + to)[i] = make_uint4(0, 0, 0, 0);
+              }
+          }
+          fence_proxy_async_smem();
+        }
       }
       if constexpr (KV) {
 #pragma unroll
