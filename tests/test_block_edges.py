@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import block_refs as ref
-from triangleops_b200 import _lib, local_block, window_attn
+from triangleops_b200 import _lib, gated_norm, local_block, rotary, window_attn
 
 gpu = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -243,3 +243,39 @@ def test_what_a_query_that_sees_nothing_holds(device, dtype, N, D, sinks, window
     ref.assert_within(out, *want["out"], "out")
     for name, got in zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, **kw)):
         ref.assert_within(got, *want[name], f"{name} {dtype}")
+
+
+def _stand_ins(monkeypatch):
+    """The launchers as graph-less functions of the CPU with gradients of the right shapes (the values take no part)."""
+    monkeypatch.setattr(window_attn.kernel, "forward", lambda q, k, v, **kw: (q * 2, q.sum(-1)))
+    monkeypatch.setattr(window_attn.kernel, "backward", lambda d, q, k, v, o, lse, **kw: (d * 2, k * 0, v * 0))
+    monkeypatch.setattr(gated_norm.kernel, "forward", lambda x, y, g, **kw: (x + y, x * 2 if kw["pre_norm"] else None, x))
+    monkeypatch.setattr(gated_norm.kernel, "backward", lambda dh, dn, x, y, g, st, **kw: dict(
+        dx=x * 2, dy=y * 2, **{"d" + w: t * 1 for w, t in kw.items() if isinstance(t, torch.Tensor)}))
+    for f in ("forward", "backward"):
+        monkeypatch.setattr(rotary.kernel, f, lambda q, k, pos, **kw: (q * 2, None if k is None else k * 2))
+
+
+def test_second_derivatives_are_refused(monkeypatch):
+    """A gradient of a gradient would lose the terms that run through the first one: an error, whether
+    the graph reaches it by the incoming gradient or by the inputs; first gradients are as they were."""
+    _stand_ins(monkeypatch)
+    x, w = torch.randn(3, 4, requires_grad=True), torch.randn(4, requires_grad=True)
+    inv, axis, pos = torch.ones(2), torch.zeros(2, dtype=torch.int32), torch.zeros(1, 1, 3, dtype=torch.int32)
+    calls = {
+        "window_attention": lambda t: window_attn.window_attention(t, t, t, window=2),
+        "gated_norm": lambda t: gated_norm.gated_norm(t, t, post_weight=w)[0],
+        "gated_norm without a second norm": lambda t: gated_norm.gated_norm(t, t, pre_norm=False)[0],
+        "rotary": lambda t: rotary.rotary(t, None, pos, inv_freq=inv, axis=axis)[0],
+    }
+    for what, f in calls.items():
+        once, = torch.autograd.grad(f(x).square().sum(), x)
+        assert not once.requires_grad and once.shape == x.shape
+        grad, = torch.autograd.grad(f(x * x).square().sum(), x, create_graph=True)
+        assert grad.requires_grad
+        with pytest.raises(RuntimeError, match="no second derivatives"):
+            torch.autograd.grad(grad.square().sum(), x)
+        if what != "rotary":  # (a turn's gradient does not depend on what is turned)
+            grad, = torch.autograd.grad(f(x).sum(), x, create_graph=True)
+            with pytest.raises(RuntimeError, match="no second derivatives"):
+                torch.autograd.grad((grad * grad).sum() + x.sum(), x)

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import torch
 
+from .. import _autograd
 from . import kernel
 
 
@@ -34,11 +35,13 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         positions, inv_freq, axis = ctx.saved_tensors
-        return (*kernel.backward(dq, dk, positions, inv_freq=inv_freq, axis=axis, interleaved=ctx.interleaved), None,
-                None, None, None)
+        grads = _autograd.first_order(
+            "rotary", lambda: kernel.backward(dq, dk, positions, inv_freq=inv_freq, axis=axis,
+                                              interleaved=ctx.interleaved), dq, dk)
+        return (*grads, None, None, None, None)
 
 
 def rotary(q, k, positions, *, inv_freq, axis, interleaved=False):
     """q and k (or None) turned by their tokens' positions
-    (:mod:`triangleops_b200.rotary.kernel` has the definition); differentiable in q and k."""
+    (:mod:`triangleops_b200.rotary.kernel` has the definition); differentiable (once) in q and k."""
     return _Rotary.apply(q, k, positions, inv_freq, axis, interleaved)
