@@ -279,3 +279,18 @@ def test_second_derivatives_are_refused(monkeypatch):
             grad, = torch.autograd.grad(f(x).sum(), x, create_graph=True)
             with pytest.raises(RuntimeError, match="no second derivatives"):
                 torch.autograd.grad((grad * grad).sum() + x.sum(), x)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("D,P", [(1024, 512), (784, 392), (768, 384), (896, 448), (1024, 100)])
+def test_rotary_of_one_wide_head(device, dtype, D, P):
+    """Many tokens a block of one head: their angles fit the block's shared memory."""
+    B, N = 2, 4800
+    g = torch.Generator(device=device).manual_seed(D)
+    q = torch.randn(B, N, 1, D, device=device, generator=g).to(dtype)
+    pos = torch.randint(-500, 500, (1, B, N), device=device, generator=g, dtype=torch.int32)
+    inv_freq, axis = rotary.frequencies(D, (P,), device=device)
+    got, _ = rotary.forward(q, None, pos, inv_freq=inv_freq, axis=axis)
+    value, size = ref.rotary(q, pos, inv_freq, axis, False)
+    ref.assert_within(got, value, ref.store(value, dtype) + 2.0**-21 * size, f"{dtype} {D}")

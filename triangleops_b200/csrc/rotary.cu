@@ -217,10 +217,12 @@ extern "C" int tops_rotary(int dtype, int64_t B, int64_t N, int64_t Hq, int64_t 
   const int64_t H = Hq + Hk, items = whole ? D / 2 / vec : interleaved ? D : D - D / 2;
   // Three items a thread or more, so that loads are ahead of the work: 1, 2, 4, 8, 16 tokens a block take
   // 96, 57, 39, 35, 31 us at 48 items a token (8 x 4096 tokens) and 82, 70, 64, 64, 70 us at 320 (2 x 8192).
-  // Few tokens: fewer a block, down to one with the heads shared by blocks, until the SMs are busy.
-  const int64_t tokens = B * N, sms = sm_count();
+  // Few tokens: fewer a block, down to one with the heads shared by blocks, until the SMs are busy. And no
+  // more than 48 KB of angles, what a block gets unasked (one token's are 4 KB at most).
+  const int64_t tokens = B * N, sms = sm_count(), most = 48 * 1024 / (P * static_cast<int64_t>(sizeof(float2)));
   a.tok = 1;
-  while (a.tok < 16 && a.tok * H * items < 3 * kRotThreads && tokens >= 4 * sms * a.tok) a.tok *= 2;
+  while (a.tok < 16 && 2 * a.tok <= most && a.tok * H * items < 3 * kRotThreads && tokens >= 4 * sms * a.tok)
+    a.tok *= 2;
   const int64_t blocks = (tokens + a.tok - 1) / a.tok;
   int64_t shares = blocks >= 2 * sms ? 1 : (2 * sms + blocks - 1) / blocks;
   shares = shares < H ? shares : H;
