@@ -294,3 +294,21 @@ def test_rotary_of_one_wide_head(device, dtype, D, P):
     got, _ = rotary.forward(q, None, pos, inv_freq=inv_freq, axis=axis)
     value, size = ref.rotary(q, pos, inv_freq, axis, False)
     ref.assert_within(got, value, ref.store(value, dtype) + 2.0**-21 * size, f"{dtype} {D}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_lengths_past_32_bits(device, dtype):
+    """A 64-bit length counts as what it is, not as its low 32 bits."""
+    B, N, D = 5, 40, 32
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(*s, generator=g).to(device, dtype) for s in ((B, 2, D), (B, N, 2, D), (B, N, 2, D)))
+    far = torch.tensor([2**32 + 3, 2**40, -(2**32) + 7, 2**31 + 1, 12], device=device)
+    near = torch.tensor([N, N, 0, N, 12], dtype=torch.int32, device=device)
+    kw = dict(window=16, sinks=1)
+    assert torch.equal(window_attn.decode(q, k, v, far, **kw), window_attn.decode(q, k, v, near, **kw))
+    old = k.clone(), v.clone()
+    window_attn.kernel.store(q, q, k, v, far)
+    for c, o in zip((k, v), old):
+        o[4, 12] = q[4]
+        assert torch.equal(c, o)

@@ -200,6 +200,14 @@ PyObject* window_attn_backward(PyObject* const* a) {
   return give_tuple(dq, dk, dv);
 }
 
+// Lengths as the kernels read them. A wider type's are brought into -1..N first (below and above it they
+// all mean the same), where their low 32 bits could be any number.
+Tensor lengths32(const Tensor& n, int64_t N) {
+  if (n.scalar_type() == at::kInt) return n.contiguous();
+  const bool wide = n.scalar_type() == at::kLong || n.is_floating_point();
+  return (wide ? n.clamp(-1, N) : n).to(at::kInt).contiguous();
+}
+
 // (q, k_cache, v_cache, lengths, window, sinks, scale) -> out
 PyObject* window_attn_decode(PyObject* const* a) {
   Tensor q = tensor(a[0]), k = tensor(a[1]), v = tensor(a[2]), n = tensor(a[3]);
@@ -219,7 +227,7 @@ PyObject* window_attn_decode(PyObject* const* a) {
   const float scale = static_cast<float>(a[6] == Py_None ? 1.0 / std::sqrt(static_cast<double>(D)) : real(a[6]));
   require_cuda(q);
   const c10::cuda::CUDAGuard guard(q.device());
-  q = rows(q), k = rows(k), v = rows(v), n = n.to(at::kInt).contiguous();
+  q = rows(q), k = rows(k), v = rows(v), n = lengths32(n, N);
   const Tensor out = like(q);
   int64_t need = 0;
   check(tops_window_attn_decode_workspace_bytes(B, N, Hq, Hkv, D, window, sinks, &need), "tops_window_attn_decode");
@@ -249,7 +257,7 @@ PyObject* window_attn_store(PyObject* const* a) {
        "k, v, the caches and lengths must be on one device");
   require_cuda(k);
   const c10::cuda::CUDAGuard guard(k.device());
-  k = rows(k), v = rows(v), n = n.to(at::kInt).contiguous();
+  k = rows(k), v = rows(v), n = lengths32(n, kc.size(1));
   const int64_t st[4] = {k.stride(0), k.stride(1), v.stride(0), v.stride(1)};
   int64_t ct[8];
   for (int i = 0; i < 4; ++i) ct[i] = kc.stride(i), ct[4 + i] = vc.stride(i);

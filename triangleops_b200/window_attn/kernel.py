@@ -53,8 +53,8 @@ def backward(dout, q, k, v, out, lse, *, window, sinks=0, scale=None, mask=None)
 def decode(q, k_cache, v_cache, lengths, *, window, sinks=0, scale=None):
     """One token for each sequence: q (B, Hq, D) stands at the last of the ``lengths[b]``
     keys that sequence has in the caches (B, N, Hkv, D), any strides, and sees the
-    ``window`` newest of them and the first ``sinks``. ``lengths`` (B,) int32 on the
-    device; a length of 0 gives zeros, one beyond N counts as N. Returns (B, Hq, D)."""
+    ``window`` newest of them and the first ``sinks``. ``lengths`` (B,) int32 (or int64, at the cost of two more
+    launches) on the device; a length of 0 gives zeros, one beyond N counts as N. Returns (B, Hq, D)."""
     if not isinstance(window, int):
         raise ValueError(f"window must be a number of keys, at least 1, got {window}")
     return _lib.bind().window_attn_decode(q, k_cache, v_cache, lengths, window, sinks, scale)
