@@ -312,3 +312,35 @@ def test_lengths_past_32_bits(device, dtype):
     for c, o in zip((k, v), old):
         o[4, 12] = q[4]
         assert torch.equal(c, o)
+
+
+@gpu
+def test_first_use_of_a_thread_inside_a_capture(device):
+    """A thread whose first call of the operators is captured into a graph, as autograd's may be."""
+    import threading
+
+    q, k, v, d = (torch.randn(1, 200, 2, 64, device=device).to(BF) for _ in range(4))
+    kw = dict(window=64, sinks=1)
+    want = window_attn.forward(q, k, v, **kw)
+    want = (*want, *window_attn.backward(d, q, k, v, *want, **kw))
+    torch.cuda.synchronize()
+    got = []
+
+    def work():
+        try:
+            graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+            with torch.cuda.graph(graph, stream=stream):
+                out, lse = window_attn.forward(q, k, v, **kw)
+                grads = window_attn.backward(d, q, k, v, out, lse, **kw)
+            graph.replay()
+            torch.cuda.synchronize()
+            got.extend(t.clone() for t in (out, lse, *grads))
+            graph.reset()
+        except Exception as e:  # noqa: BLE001
+            got.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    assert not isinstance(got[0], Exception), got
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

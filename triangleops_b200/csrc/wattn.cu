@@ -443,14 +443,15 @@ __global__ void __launch_bounds__(WattnFwdCfg<DT>::THREADS, 2)
 // host side
 // ---------------------------------------------------------------------------
 // A thread that has not used its device yet (autograd has threads of its own) has no current context,
-// without which a tensor map cannot be encoded; the first runtime call that needs one makes it.
+// without which a tensor map cannot be encoded. cudaSetDevice makes it current, and is open while a stream
+// is captured, as memory calls are not.
 static void bind_context() {
   static thread_local uint64_t bound = 0;
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = uint64_t(1) << (dev & 63);
   if (bound & bit) return;
-  cudaFree(nullptr);
+  cudaSetDevice(dev);
   bound |= bit;
 }
 
