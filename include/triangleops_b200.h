@@ -256,7 +256,8 @@ int tops_transition_forward(int dtype, int64_t M, int64_t C, const void* x, cons
  * and whose norms are folded into its projections): windowed attention with sinks, the norms
  * around a block fused with its gate and residual scale, rotary positions. dtype: TOPS_F16,
  * TOPS_BF16 or TOPS_F32. Strides count elements; pointers need only their type's alignment
- * unless noted; zero sizes return TOPS_OK without a launch. */
+ * unless noted. Zero sequences, tokens or rows return TOPS_OK without a kernel: no other input is read, and
+ * outputs that sum over them are set to zero. */
 
 /* out = softmax(scale q k^T) v, where query i, at key position p = i + Nk - Nq, sees key j iff
  *   j <= p + right  and  (j >= p - left  or  j < sinks)  and  (mask == NULL or mask[b*Nk + j]).
@@ -271,8 +272,7 @@ int tops_window_attn_forward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64
                              void* stream);
 /* Gradients dq [B][Nq][Hq][D], dk and dv [B][Nk][Hkv][D] from dout (dout_strides[3] = {b, n, h})
  * and the forward's out and lse. workspace: 16-byte aligned, of the size that
- * tops_window_attn_backward_workspace_bytes gives. Bitwise repeatable. Nq = 0 sets dk and dv to zero
- * and reads none of the other pointers. */
+ * tops_window_attn_backward_workspace_bytes gives. Bitwise repeatable. */
 int tops_window_attn_backward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
                               const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask,
                               int64_t left, int64_t right, int64_t sinks, float scale, const void* dout,

@@ -344,3 +344,30 @@ def test_first_use_of_a_thread_inside_a_capture(device):
     t.join()
     assert not isinstance(got[0], Exception), got
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_no_rows_in_c():
+    """Zero rows are no error at the gated norm's C entries, and nothing has to be there."""
+    need = ctypes.c_int64(-1)
+    assert _c("tops_gated_norm_backward_workspace_bytes", 0, 3, 64, ctypes.byref(need)) == _lib.OK and need.value == 0
+    none = [None] * 6
+    assert _c("tops_gated_norm_forward", _lib.BF16, _lib.BF16, 0, 3, 64, 1, 1, 1, 1e-5, None, 64, None, 64, None, 64, *none[:5],
+              None, None, None, None) == _lib.OK
+    assert _c("tops_gated_norm_backward", _lib.BF16, _lib.F32, 0, 3, 64, 1, 1, 1, None, 64, None, 64, None, 64, None, 64,
+              None, 64, *([None] * 15)) == _lib.OK
+    assert _c("tops_window_attn_decode_workspace_bytes", 2, 0, 4, 2, 64, 9000, 0, ctypes.byref(need)) == _lib.OK
+    assert need.value == 0
+
+
+@gpu
+def test_no_rows_on_the_device(device):
+    w = [torch.full((64,), float("nan"), device=device) for _ in range(5)]
+    gate = torch.full((3, 64), float("nan"), dtype=BF, device=device)
+    assert _c("tops_gated_norm_backward", _lib.BF16, _lib.F32, 0, 3, 64, 1, 1, 1, None, 64, None, 64, None, 64, None, 64, None,
+              64, *([None] * 7), gate, *w, None, ctypes.c_void_p(_lib.stream_ptr())) == _lib.OK
+    assert not any(t.any() for t in (gate, *w))
+    k = torch.zeros(2, 0, 2, 64, dtype=BF, device=device)
+    n = torch.tensor([0, 5], dtype=torch.int32, device=device)
+    q = torch.ones(2, 4, 64, dtype=BF, device=device)
+    assert not window_attn.decode(q, k, k, n, window=9000).any()
+    window_attn.kernel.store(q[:, :2], q[:, 2:], k, k, n)

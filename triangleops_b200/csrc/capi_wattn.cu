@@ -127,10 +127,9 @@ extern "C" int tops_window_attn_backward_workspace_bytes(int dtype, int64_t B, i
 extern "C" int tops_window_attn_decode_workspace_bytes(int64_t B, int64_t N, int64_t Hq, int64_t Hkv, int64_t D,
                                                        int64_t window, int64_t sinks, int64_t* bytes) {
   if (bytes == nullptr || window < 1 || sinks < 0) return TOPS_ERR_ARG;
-  if (N < 1) return TOPS_ERR_SHAPE;
   if (const int rc = wattn_sizes(B, N, Hq, Hkv, D)) return rc;
   // a plan divides the SMs among the sequences
-  *bytes = B == 0 ? 0 : wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
+  *bytes = B == 0 || N == 0 ? 0 : wattn_decode_plan(B, N, Hq, Hkv, D, window, sinks).part * 4;
   return TOPS_OK;
 }
 
@@ -139,8 +138,15 @@ extern "C" int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t 
                                        const int32_t* lengths, int64_t window, int64_t sinks, float scale,
                                        void* workspace, void* out, void* stream) {
   if (dtype != TOPS_BF16 && dtype != TOPS_F16 && dtype != TOPS_F32) return TOPS_ERR_DTYPE;
-  if (window < 1) return TOPS_ERR_ARG;
-  if (N < 1) return TOPS_ERR_SHAPE;
+  if (window < 1 || sinks < 0) return TOPS_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (N == 0) {  // caches without a place: no sequence has a key
+    if (const int rc = wattn_sizes(B, N, Hq, Hkv, D)) return rc;
+    if (B == 0) return TOPS_OK;
+    if (out == nullptr) return TOPS_ERR_ARG;
+    const size_t bytes = static_cast<size_t>(B) * Hq * D * (dtype == TOPS_F32 ? 4 : 2);
+    return cudaMemsetAsync(out, 0, bytes, st) == cudaSuccess ? TOPS_OK : TOPS_ERR_CUDA;
+  }
   WattnArgs a;
   if (strides == nullptr) return TOPS_ERR_ARG;
   const int64_t full[9] = {strides[0], 0,          strides[1], strides[2], strides[3],
@@ -149,7 +155,6 @@ extern "C" int tops_window_attn_decode(int dtype, int64_t B, int64_t N, int64_t 
   if (B == 0) return TOPS_OK;
   if (lengths == nullptr || out == nullptr) return TOPS_ERR_ARG;
   a.lengths = lengths;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype != TOPS_F32 && D % 8 == 0 && D <= 128 && wattn_decode_rows(q, a.qs[0], a.qs[2], 0) &&
       wattn_decode_rows(k, a.ks[0], a.ks[1], a.ks[2]) && wattn_decode_rows(v, a.vs[0], a.vs[1], a.vs[2])) {
     float* part = static_cast<float*>(workspace);

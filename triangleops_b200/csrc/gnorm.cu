@@ -670,8 +670,16 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
                                         void* dpre_b, void* workspace, void* stream) {
   if (dtype != TOPS_BF16 && dtype != TOPS_F16 && dtype != TOPS_F32) return TOPS_ERR_DTYPE;
   if (w_dtype != dtype && w_dtype != TOPS_F32) return TOPS_ERR_DTYPE;
-  if (rows <= 0 || C <= 0 || C > kGnMostC || groups <= 0 || rows % groups != 0 || rows >= (int64_t(1) << 30))
+  if (rows < 0 || C <= 0 || C > kGnMostC || groups <= 0 || rows % groups != 0 || rows >= (int64_t(1) << 30))
     return TOPS_ERR_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {  // sums of nothing
+    const size_t w_bytes = C * (w_dtype == TOPS_F32 ? 4 : 2), g_bytes = groups * C * (dtype == TOPS_F32 ? 4 : 2);
+    bool ok = dgate == nullptr || cudaMemsetAsync(dgate, 0, g_bytes, st) == cudaSuccess;
+    for (void* w : {dpost_w, dpost_b, dres_s, dpre_w, dpre_b})
+      ok = ok && (w == nullptr || cudaMemsetAsync(w, 0, w_bytes, st) == cudaSuccess);
+    return ok ? TOPS_OK : TOPS_ERR_CUDA;
+  }
   if (x == nullptr || y == nullptr || stats == nullptr || dx == nullptr || dy == nullptr || workspace == nullptr ||
       (gate != nullptr && dgate == nullptr))
     return TOPS_ERR_ARG;
@@ -697,7 +705,6 @@ extern "C" int tops_gated_norm_backward(int dtype, int w_dtype, int64_t rows, in
   auto fits = [&](const void* q, int64_t stride) { return gn_pieces(q, stride, vec, bytes); };
   const bool whole = fits(x, xs) && fits(y, ys) && fits(gate, gs) && fits(dh, dhs) && fits(dn, dns) && fits(dx, C) &&
                      fits(dy, C) && fits(dgate, C);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   const GnormShape& g = p.bwd;
   const size_t smem = (static_cast<size_t>(4 * g.tpr) + (g.slots > 1 ? g.threads : 0)) * p.v * 4;
   auto run = [&](auto t, auto w, auto v, auto tpr) {
