@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import block_refs as ref
-from triangleops_b200 import _lib, gated_norm, local_block, rotary, window_attn
+from triangleops_b200 import _build, _lib, gated_norm, local_block, rotary, window_attn
 
 gpu = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -371,3 +371,15 @@ def test_no_rows_on_the_device(device):
     q = torch.ones(2, 4, 64, dtype=BF, device=device)
     assert not window_attn.decode(q, k, k, n, window=9000).any()
     window_attn.kernel.store(q[:, :2], q[:, 2:], k, k, n)
+
+
+def test_the_extension_is_of_this_torch(monkeypatch, tmp_path):
+    """Another torch or Python than the one that it was compiled against, or none on record: built again."""
+    _lib.bind()
+    assert not _build.needs_bind()
+    monkeypatch.setattr(torch, "__version__", "0.0.1")
+    assert _build.needs_bind()
+    monkeypatch.undo()
+    assert not _build.needs_bind()
+    monkeypatch.setattr(_build, "BIND_STAMP", str(tmp_path / "none"))
+    assert _build.needs_bind()

@@ -22,6 +22,7 @@ LIB_NAME = "libtriangleops_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 BIND_SRC = os.path.join(CSRC, "bind.cpp")
 BIND_PATH = os.path.join(HERE, "_bind.so")
+BIND_STAMP = BIND_PATH + ".for"  # what _bind.so was compiled against
 
 NVCC_FLAGS = [
     "-gencode",
@@ -59,12 +60,23 @@ def needs_build() -> bool:
     return any(os.path.getmtime(s) > t for s in _sources())
 
 
+def _bind_against() -> str:
+    import torch
+
+    return f"torch {torch.__version__}, Python {sys.version_info.major}.{sys.version_info.minor}"
+
+
 def needs_bind() -> bool:
-    if not os.path.exists(BIND_PATH):
+    """Whether ``_bind.so`` is missing, older than its sources, or of another torch or Python than
+    this process's (whose C++ interfaces it would call as if they were its own)."""
+    if not os.path.exists(BIND_PATH) or not os.path.exists(BIND_STAMP):
         return True
+    with open(BIND_STAMP) as f:
+        if f.read() != _bind_against():
+            return True
     header = os.path.join(HERE, "..", "include", "triangleops_b200.h")
     t = os.path.getmtime(BIND_PATH)
-    return any(os.path.exists(s) and os.path.getmtime(s) > t for s in (BIND_SRC, header))
+    return any(os.path.exists(s) and os.path.getmtime(s) > t for s in (BIND_SRC, os.path.join(CSRC, "status.h"), header))
 
 
 def _run(cmd: list[str], tmp: str, path: str, verbose: bool) -> None:
@@ -95,6 +107,8 @@ def build_bind(verbose: bool = False, force: bool = False) -> str:
            tmp, f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
     _run(cmd, tmp, BIND_PATH, verbose)
+    with open(BIND_STAMP, "w") as f:
+        f.write(_bind_against())
     return BIND_PATH
 
 
