@@ -272,7 +272,9 @@ int tops_window_attn_forward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64
                              void* stream);
 /* Gradients dq [B][Nq][Hq][D], dk and dv [B][Nk][Hkv][D] from dout (dout_strides[3] = {b, n, h})
  * and the forward's out and lse. workspace: 16-byte aligned, of the size that
- * tops_window_attn_backward_workspace_bytes gives. Bitwise repeatable. */
+ * tops_window_attn_backward_workspace_bytes gives: two floats a query (Nq rounded up to 128, and 64), and
+ * where queries lie past the sinks' windows, for each key head 2 (1 + Hq / Hkv) fp32 rows a sink and up to
+ * 1 MB more for each SM. Bitwise repeatable. */
 int tops_window_attn_backward(int dtype, int64_t B, int64_t Nq, int64_t Nk, int64_t Hq, int64_t Hkv, int64_t D,
                               const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask,
                               int64_t left, int64_t right, int64_t sinks, float scale, const void* dout,

@@ -383,3 +383,32 @@ def test_the_extension_is_of_this_torch(monkeypatch, tmp_path):
     assert not _build.needs_bind()
     monkeypatch.setattr(_build, "BIND_STAMP", str(tmp_path / "none"))
     assert _build.needs_bind()
+
+
+@pytest.mark.parametrize("B,N,Hq,Hkv,D,left,sinks", [(1, 131072, 4, 1, 128, 1, 8192), (2, 65536, 32, 8, 128, 1, 8192),
+                                                     (4, 8192, 16, 4, 64, 511, 4), (1, 2**20, 8, 8, 128, 1023, 128),
+                                                     (1, 300, 2, 2, 32, 9, 40)])
+def test_backward_workspace_with_sinks(B, N, Hq, Hkv, D, left, sinks):
+    """What the header says of it, at 148 SMs: the sinks' parts do not grow with the queries without limit."""
+    need = ctypes.c_int64(0)
+    assert _c("tops_window_attn_backward_workspace_bytes", _lib.BF16, B, N, N, Hq, Hkv, D, left, 0, sinks,
+              ctypes.byref(need)) == _lib.OK
+    stats = 2 * B * Hq * (-(-N // 128) * 128 + 64) * 4 + 16
+    rows = -(-sinks // 128) * 128  # (whole tiles of sinks)
+    parts = B * Hkv * 2 * (1 + Hq // Hkv) * rows * max(64, D) * 4 + 148 * 2**20
+    assert stats <= need.value <= stats + parts
+
+
+@gpu
+def test_many_sinks_and_late_queries(device):
+    """So many sinks and queries that a block of late queries walks more than its share of a tile's own."""
+    B, N, H, D, sinks = 2, 7000, 8, 32, 300
+    g = torch.Generator(device=device).manual_seed(1)
+    q, k, v, d = (torch.randn(B, N, H, D, device=device, generator=g).to(BF) for _ in range(4))
+    kw = dict(window=2, sinks=sinks)
+    out, lse = window_attn.forward(q, k, v, **kw)
+    grads = window_attn.backward(d, q, k, v, out, lse, **kw)
+    at = (slice(1, 2), slice(None), slice(5, 6))
+    want = ref.attention(q[at], k[at], v[at], 2, sinks, dout=d[at])
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        ref.assert_within(got[at], *want[name], name)

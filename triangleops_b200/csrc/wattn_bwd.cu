@@ -680,8 +680,17 @@ inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
   late = late < 0 ? 0 : late > Nq ? Nq : late;
   const int64_t blocks = p.nsb > 0 && late < Nq ? (Nq - late / 8 * 8 + 63) / 64 : 0;
   const int64_t own = group * ((static_cast<int64_t>(a.left) + a.right + 128 + 63) / 64);
-  p.per = static_cast<int>(own / 4 < 4 ? 4 : own / 4);
-  p.nx = static_cast<int>((blocks + p.per - 1) / p.per);
+  int64_t per = own / 4 < 4 ? 4 : own / 4;
+  // ..but no more blocks than 8 for each SM, where that many sinks alone do not make them: each leaves a
+  // fp32 part of up to 128 KB (8192 sinks, a window of 2, 4 query heads to a key head, 131072 queries: 17 GB
+  // a key head without this, 142 MB so)
+  const int64_t units = static_cast<int64_t>(a.B) * a.Hkv * p.nsb * group, room = units > 0 ? 8 * sm_count() / units : 0;
+  if (room < 1)
+    per = blocks > per ? blocks : per;
+  else if (per * room < blocks)
+    per = (blocks + room - 1) / room;
+  p.per = static_cast<int>(per);
+  p.nx = static_cast<int>((blocks + per - 1) / per);
   if (p.nx == 0) p.nsb = 0;
   const int64_t DT = a.D <= 64 ? 64 : 128;
   p.part = static_cast<int64_t>(a.B) * a.Hkv * p.nsb * (1 + static_cast<int64_t>(group) * p.nx) * 2 * p.keep * DT;
