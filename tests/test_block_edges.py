@@ -412,3 +412,72 @@ def test_many_sinks_and_late_queries(device):
     want = ref.attention(q[at], k[at], v[at], 2, sinks, dout=d[at])
     for name, got in zip(("dq", "dk", "dv"), grads):
         ref.assert_within(got[at], *want[name], name)
+
+
+def _odd(t):
+    """The same values one element off 16 bytes, rows an odd number of elements apart."""
+    flat = torch.zeros(t.numel() // t.shape[-1], t.shape[-1] + 3, dtype=t.dtype, device=t.device)
+    flat[:, 1:-2] = t.reshape(-1, t.shape[-1])
+    return flat[:, 1:-2].view(t.shape)
+
+
+def _part(t):
+    """The same values as a part of wider rows, which 16-byte loads can follow."""
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 64, dtype=t.dtype, device=t.device)
+    wide[..., 32:-32] = t
+    return wide[..., 32:-32]
+
+
+def _channels_first(t):
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+def _one_row(t):
+    """Its first row for all, by a stride of zero."""
+    return t.reshape(-1, t.shape[-1])[:1].expand(t.numel() // t.shape[-1], t.shape[-1]).view(t.shape)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("C", [128, 771])
+@pytest.mark.parametrize("lay", [_odd, _part, _channels_first, _one_row])
+@pytest.mark.parametrize("which", ["x", "y", "gate", "dh", "dn", "all"])
+def test_gated_norm_strides(device, dtype, C, lay, which):
+    """Each input by itself, and all of them, in other strides: values forward and backward. Bounds: the
+    store, fp32 arithmetic of 2^-17 of the largest value that takes part, of a root of T such terms in sums."""
+    T = 60
+    g = torch.Generator().manual_seed(C)
+    t = {n: (torch.randn(3, T // 3, C, generator=g) * (2.0 if n == "x" else 1.0)).to(device, dtype)
+         for n in ("x", "y", "gate", "dh", "dn")}
+    par = {n: (torch.randn(C, generator=g) * 0.2 + (not n.endswith("bias"))).to(device, dtype)
+           for n in ("post_weight", "post_bias", "res_scale", "pre_weight", "pre_bias")}
+    for n in t:
+        if which in (n, "all"):
+            t[n] = lay(t[n])
+    want = ref.gated_norm(t["x"], t["y"], t["gate"], par, "layer", 1e-5, dh=t["dh"], dn=t["dn"])
+    h, n, stats = gated_norm.forward(t["x"], t["y"], t["gate"], **par)
+    got = {"h": h, "n": n, **gated_norm.backward(t["dh"], t["dn"], t["x"], t["y"], t["gate"], stats, **par)}
+    for name, value in want.items():
+        terms = T if name[1:] in par else 1
+        size = max(4.0, value.abs().max().item(), *(v.abs().max().item() for v in want.values() if v.dim() > 1))
+        ref.assert_within(got[name], value, ref.store(value, dtype) + 2.0**-17 * size * terms**0.5, f"{name} {which}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("lay", [_odd, _part, lambda t: t.transpose(1, 2).contiguous().transpose(1, 2),
+                                 lambda t: t[:, :1].expand_as(t)])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout", "all"])
+def test_window_attention_strides(device, dtype, lay, which):
+    """Each input by itself in other strides, with gradients."""
+    g = torch.Generator().manual_seed(4)
+    t = {n: torch.randn(2, 150, 2 if n in "kv" else 4, 64, generator=g).to(device, dtype) for n in ("q", "k", "v", "dout")}
+    for n in t:
+        if which in (n, "all"):
+            t[n] = lay(t[n])
+    q, k, v, d = t.values()
+    want = ref.attention(q, k, v, (40, 9), 3, dout=d)
+    out, lse = window_attn.forward(q, k, v, window=(40, 9), sinks=3)
+    ref.assert_within(out, *want["out"], "out")
+    for name, got in zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, window=(40, 9), sinks=3)):
+        ref.assert_within(got, *want[name], name)
