@@ -32,7 +32,7 @@
 //
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the
-// end, has -lse2 = -inf, so that its P is 0; (KV) its rows of the q and dO tiles are zeroed likewise.
+// end, has -lse2 = -inf, so that its P is 0; (KV, with a mask) its rows of the q and dO tiles are zeroed likewise.
 #include <algorithm>
 #include "sm100.cuh"
 #include "wattn.h"
@@ -169,7 +169,7 @@ struct WattnWalk {
   }
 };
 
-template <typename T, int DT, bool KV>
+template <typename T, int DT, bool KV, bool MASK>
 __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, const CUtensorMap& map_a2,
                                                      const CUtensorMap& map_b1, const CUtensorMap& map_b2,
                                                      const WattnBwdArgs& a) {
@@ -306,7 +306,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
       hi = at + a.left + 1;
       if (at < a.sinks) hi = walk.slot == 0 ? walk.late + off : a.Nk;
       if (walk.slot > 0) lo = max(lo, walk.late + off);
-      if (a.mask && at < a.Nk) keep = a.mask[static_cast<int64_t>(walk.b) * a.Nk + at] != 0;
+      if (MASK && at < a.Nk) keep = a.mask[static_cast<int64_t>(walk.b) * a.Nk + at] != 0;
     } else {
       const int p = at + off;
       lo = p - a.left;
@@ -326,7 +326,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
       next = walk.row_after(next, it);
       uint32_t kept = 0xffffffffu;
       bool whole = keep;
-      if (!KV && a.mask) {
+      if (!KV && MASK) {
         const int k = r0 + lane;
         const uint8_t byte = k < a.Nk ? a.mask[static_cast<int64_t>(walk.b) * a.Nk + k] : 0;
         kept = __ballot_sync(0xffffffffu, byte != 0);
@@ -384,28 +384,26 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
         for (int i = 0; i < 32; ++i)
           if (!(see >> i & 1)) x[i] = 0u;
       }
-      if (KV && a.mask && wq == 0) {
-        // T1 and T2 of this tile are done: rows of queries that see nothing may be zeroed for P^T dO and
-        // dS^T q, so that no NaN there meets a P of 0
-        const bool none = sm.st[r][0][32 * g + lane] == -INFINITY;
-        if (__any_sync(0xffffffffu, none)) {
-          if (none) {
-#pragma unroll
-            for (int u = 0; u < SUB; ++u)
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int to = u * 64 * 128 + (32 * g + lane) * 128;
-                reinterpret_cast<uint4*>(sm.b1[r] + to)[i] = make_uint4(0, 0, 0, 0);
-                reinterpret_cast<uint4*>(sm.b2[r] + to)[i] = make_uint4(0, 0, 0, 0);
-              }
-          }
-          fence_proxy_async_smem();
-        }
-      }
       if constexpr (KV) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) pk[i] = E::pack2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
         tmem_st16(t1, pk);
+        if (MASK && edge && wq == 0) {
+          // T1 and T2 of this tile are done: rows of queries that see nothing may be zeroed for P^T dO and
+          // dS^T q, so that no NaN there meets a P of 0 (without an edge each of them sees the warp's keys).
+          // Here, where few registers are in use: before P it cost a spill
+          const bool none = sm.st[r][0][32 * g + lane] == -INFINITY;
+          if (__any_sync(0xffffffffu, none)) {
+            if (none)
+#pragma unroll 1
+              for (int i = 0; i < 8 * SUB; ++i) {
+                const int to = (i >> 3) * 64 * 128 + (32 * g + lane) * 128 + (i & 7) * 16;
+                *reinterpret_cast<uint4*>(sm.b1[r] + to) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(sm.b2[r] + to) = make_uint4(0, 0, 0, 0);
+              }
+            fence_proxy_async_smem();
+          }
+        }
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -442,7 +440,7 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
         pk[i] = E::pack2(r0, r1);
       }
       tmem_st16(t2 + 16, pk);
-      if (!KV && a.mask && !whole && wq == 0) {
+      if (!KV && MASK && !whole && wq == 0) {
         // T1 of this tile is done: its masked keys' rows may be zeroed for dS k
         if (!(kept >> lane & 1)) {
 #pragma unroll
@@ -515,38 +513,41 @@ __device__ __forceinline__ void wattn_backward_block(const CUtensorMap& map_a1, 
 }
 
 // Both kinds of block in one launch, KV's first: Q's fill the SMs that the last KV blocks leave. Maps:
-// boxes of 64 rows.
-template <typename T, int DT>
+// boxes of 64 rows. MASK: there is a key mask (its code in the way of a call without one costs 0.3 us of
+// 16.5, 1024 queries of 4 heads forward and backward).
+template <typename T, int DT, bool MASK>
 __global__ void __launch_bounds__(WattnBwdCfg<DT>::THREADS, 1)
     wattn_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_d,
                           const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                           const __grid_constant__ WattnBwdArgs a) {
   if (static_cast<int>(blockIdx.x) < a.kv_blocks)
-    wattn_backward_block<T, DT, true>(map_k, map_v, map_q, map_d, a);
+    wattn_backward_block<T, DT, true, MASK>(map_k, map_v, map_q, map_d, a);
   else
-    wattn_backward_block<T, DT, false>(map_q, map_d, map_k, map_v, a);
+    wattn_backward_block<T, DT, false, MASK>(map_q, map_d, map_k, map_v, a);
 }
 
 // -delta, delta = sum_d dO O, and -lse2 = -lse log2(e) (f16: + 14) per query, in rows of nqp: queries past
 // Nq, and those that see nothing, get -inf and 0. f16: the largest |dO|^2 of those that see something, and
 // (blocks behind the queries') the largest |v|^2 of the keys that the mask keeps, of `keys` from `key0` on
-// and of the sinks before them. Eight threads a row, 16-byte loads.
+// and of the sinks before them. Eight threads a row, 16-byte loads. Blocks: 32 rows in x, heads in y,
+// sequences in z, of which a grid has 65535 at most: these go on by the grid. (All three in x, taken apart by
+// divisions, cost 0.9 us a call, of 21 for 1024 queries of 4 heads forward and backward.)
 template <typename T, int DT>
 __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* __restrict__ dout, int64_t s0,
                                                           int64_t s1, int64_t s2, const T* __restrict__ out,
-                                                          const float* __restrict__ lse, int nqp, unsigned q_blocks,
-                                                          int key0, int keys, float* __restrict__ lse2,
-                                                          float* __restrict__ delta, unsigned* __restrict__ top) {
+                                                          const float* __restrict__ lse, int nqp, int key0, int keys,
+                                                          float* __restrict__ lse2, float* __restrict__ delta,
+                                                          unsigned* __restrict__ top) {
   using E = Elem<T>;
   constexpr bool TOP = E::kFmt == 0;
   pdl_trigger();
   const int part = threadIdx.x & 7, in = threadIdx.x >> 3;
-  auto load = [&](const T* p, uint4* u) {
+  auto load = [&](const T* p, bool there, uint4* u) {
 #pragma unroll
     for (int k = 0; k < DT / 64; ++k) {
       const int c = part * 8 + 64 * k;
       u[k] = make_uint4(0, 0, 0, 0);
-      if (c < a.D) u[k] = *reinterpret_cast<const uint4*>(p + c);
+      if (there && c < a.D) u[k] = *reinterpret_cast<const uint4*>(p + c);
     }
   };
   auto dot = [&](const uint4* u, const uint4* w) {
@@ -561,53 +562,44 @@ __global__ void __launch_bounds__(256) wattn_stats_kernel(WattnArgs a, const T* 
     for (int o = 4; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
   };
-  uint4 u[DT / 64], w[DT / 64];
-  float size = 0.f;  // |dO|^2 or |v|^2 of the row
-  // blocks of 32 queries, then heads, then sequences: all in x, whose range the tiles' grid shares
-  if (!TOP || blockIdx.x < q_blocks) {
-    const unsigned blocks = nqp / 32;
-    const int i = static_cast<int>(blockIdx.x % blocks * 32 + in);
-    const int64_t bh = blockIdx.x / blocks;
-    const int h = static_cast<int>(bh % a.Hq), b = static_cast<int>(bh / a.Hq);
-    float x = 0.f, v = -INFINITY;
-    if (i < a.Nq) {
-      load(dout + b * s0 + i * s1 + h * s2, u);
-      load(out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D, w);
-      v = lse[bh * a.Nq + i];
-    } else {
-#pragma unroll
-      for (int k = 0; k < DT / 64; ++k) u[k] = w[k] = make_uint4(0, 0, 0, 0);
+  const int q_blocks = nqp / 32, block = blockIdx.x;
+  const bool of_v = TOP && block >= q_blocks;
+  const int i = (of_v ? block - q_blocks : block) * 32 + in, heads = of_v ? a.Hkv : a.Hq;
+  const int sinks = min(a.sinks, key0), j = i < sinks ? i : key0 + i - sinks;
+  unsigned bits = 0;
+  for (int b = blockIdx.z; b < a.B; b += gridDim.z)
+    for (int h = blockIdx.y; h < heads; h += gridDim.y) {
+      uint4 u[DT / 64], w[DT / 64];
+      float size = 0.f;  // |dO|^2 or |v|^2 of the row
+      if (!of_v) {
+        const int64_t bh = static_cast<int64_t>(b) * a.Hq + h;
+        const bool there = i < a.Nq;
+        load(dout + b * s0 + i * s1 + h * s2, there, u);
+        load(out + ((static_cast<int64_t>(b) * a.Nq + i) * a.Hq + h) * a.D, there, w);
+        const float v = there && part == 0 ? lse[bh * a.Nq + i] : -INFINITY, x = dot(u, w);
+        if (TOP) size = dot(u, u);
+        if (v == -INFINITY) size = 0.f;  // (the row's other threads count nothing)
+        if (part == 0) {
+          lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : wattn_lift<T>() - v * kLog2e;
+          delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
+        }
+      } else {
+        const bool there = i < keys && (a.mask == nullptr || a.mask[static_cast<int64_t>(b) * a.Nk + j] != 0);
+        load(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + h * a.vs[2], there, u);
+        size = dot(u, u);
+      }
+      // what is not finite makes the results so wherever it goes, and says nothing of the others' size
+      if (TOP && size < INFINITY) bits = max(bits, __float_as_uint(size));
     }
-    x = dot(u, w);
-    if (TOP) size = dot(u, u);
-    if (v == -INFINITY) size = 0.f;
-    if (part == 0) {
-      lse2[bh * nqp + i] = v == -INFINITY ? -INFINITY : wattn_lift<T>() - v * kLog2e;
-      delta[bh * nqp + i] = v == -INFINITY ? 0.f : -x;
-    }
-  } else {
-    const unsigned blocks = (keys + 31) / 32, unit = blockIdx.x - q_blocks;
-    const int i = static_cast<int>(unit % blocks * 32 + in), sinks = min(a.sinks, key0);
-    const int64_t bh = unit / blocks;
-    const int h = static_cast<int>(bh % a.Hkv), b = static_cast<int>(bh / a.Hkv);
-    const int j = i < sinks ? i : key0 + i - sinks;
-    const bool there = i < keys && (a.mask == nullptr || a.mask[static_cast<int64_t>(b) * a.Nk + j] != 0);
-#pragma unroll
-    for (int k = 0; k < DT / 64; ++k) u[k] = make_uint4(0, 0, 0, 0);
-    if (there) load(static_cast<const T*>(a.v) + b * a.vs[0] + j * a.vs[1] + h * a.vs[2], u);
-    size = dot(u, u);
-  }
   if constexpr (TOP) {
-    // what is not finite makes the results so wherever it goes, and says nothing of the others' size
-    unsigned bits = size < INFINITY ? __float_as_uint(size) : 0u;
     bits = __reduce_max_sync(0xffffffffu, bits);
     __shared__ unsigned most[8];
     if ((threadIdx.x & 31) == 0) most[threadIdx.x >> 5] = bits;
     __syncthreads();
     if (threadIdx.x == 0) {
 #pragma unroll
-      for (int i = 1; i < 8; ++i) bits = max(bits, most[i]);
-      unsigned* t = top + (blockIdx.x < q_blocks ? 0 : 1);
+      for (int k = 1; k < 8; ++k) bits = max(bits, most[k]);
+      unsigned* t = top + of_v;
       if (bits > *reinterpret_cast<volatile unsigned*>(t)) atomicMax(t, bits);  // (a maximum has no order)
     }
   }
@@ -627,8 +619,9 @@ __global__ void __launch_bounds__(256) wattn_parts_kernel(const WattnBwdArgs a) 
   const int at = threadIdx.x % (W::PER * W::ROWS), share = threadIdx.x / (W::PER * W::ROWS);
   const unsigned pairs = (a.keep + W::ROWS - 1) / W::ROWS, unit = blockIdx.x / pairs;
   const int row = blockIdx.x % pairs * W::ROWS + at / W::PER, col = at % W::PER * 8;
-  const int which = unit & 1, kb = (unit >> 1) % a.nsb;
-  const int64_t bh = (unit >> 1) / a.nsb;
+  const unsigned nsb = a.nsb, which = unit & 1;
+  const int kb = static_cast<int>((unit >> 1) % nsb);
+  const int64_t bh = (unit >> 1) / nsb;
   const int key = kb * 128 + row;
   const bool live = row < a.keep && key < a.sinks && col < a.D;
   const int n = live ? 1 + a.group * a.nx : 0;
@@ -697,7 +690,7 @@ inline WattnBwdPlan wattn_bwd_plan(const WattnArgs& a, int64_t Nq) {
   return p;
 }
 
-template <typename T, int DT>
+template <typename T, int DT, bool MASK>
 static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
                           const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
   bind_context();
@@ -723,19 +716,18 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
   unsigned* top = reinterpret_cast<unsigned*>(ws + 2 * p.stats);
   const bool f16 = dtype == TOPS_F16;
   const int key0 = std::max(0, a.Nk - a.Nq - a.left), keys = a.Nk - key0 + std::min(a.sinks, key0);
-  const int64_t q_blocks = static_cast<int64_t>(a.B) * a.Hq * (p.nqp / 32);
-  const int64_t stats = q_blocks + (f16 ? heads * ((keys + 31) / 32) : 0);
+  const dim3 stats(p.nqp / 32 + (f16 ? (keys + 31) / 32 : 0), std::min(a.Hq, 65535), std::min(a.B, 65535));
   constexpr int ROWS = WattnParts<DT>::ROWS;
   const int64_t parts = heads * 2 * p.nsb * ((p.keep + ROWS - 1) / ROWS);
-  if (std::max(std::max(grid, stats), parts) >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
+  if (std::max(grid, parts) >= (int64_t(1) << 31)) return TOPS_ERR_SHAPE;
   f.own = static_cast<int>(own), f.kv_blocks = static_cast<int>(kv), f.dq = dq, f.dk = dk, f.dv = dv;
   if (f16 && cudaMemsetAsync(top, 0, 8, st) != cudaSuccess) return TOPS_ERR_CUDA;
   f.top = top;
-  wattn_stats_kernel<T, DT><<<static_cast<unsigned>(stats), 256, 0, st>>>(
-      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp,
-      static_cast<unsigned>(q_blocks), key0, keys, lse2, delta, top);
+  wattn_stats_kernel<T, DT><<<stats, 256, 0, st>>>(
+      a, static_cast<const T*>(dout), ds[0], ds[1], ds[2], static_cast<const T*>(out), lse, p.nqp, key0, keys, lse2,
+      delta, top);
   const size_t smem = sizeof(WattnBwdSmem<DT>) + 1024;
-  auto kern = wattn_backward_kernel<T, DT>;
+  auto kern = wattn_backward_kernel<T, DT, MASK>;
   static std::atomic<uint64_t> done{0};
   set_smem_once(kern, smem, done);
   launch_pdl(kern, static_cast<unsigned>(grid), WattnBwdCfg<DT>::THREADS, smem, st, mq, md, mk, mv, f);
@@ -746,8 +738,14 @@ static int launch_wattn_backward(int dtype, const WattnArgs& a, const void* dout
 template <typename T>
 int run_wattn_backward(int dtype, const WattnArgs& a, const void* dout, const int64_t* ds, const void* out,
                        const float* lse, float* ws, void* dq, void* dk, void* dv, cudaStream_t st) {
-  return a.D <= 64 ? launch_wattn_backward<T, 64>(dtype, a, dout, ds, out, lse, ws, dq, dk, dv, st)
-                   : launch_wattn_backward<T, 128>(dtype, a, dout, ds, out, lse, ws, dq, dk, dv, st);
+  const auto run = [&](auto dt, auto mask) {
+    return launch_wattn_backward<T, decltype(dt)::value, decltype(mask)::value>(dtype, a, dout, ds, out, lse, ws, dq, dk, dv,
+                                                                                st);
+  };
+  using std::integral_constant;
+  if (a.D <= 64)
+    return a.mask ? run(integral_constant<int, 64>(), std::true_type()) : run(integral_constant<int, 64>(), std::false_type());
+  return a.mask ? run(integral_constant<int, 128>(), std::true_type()) : run(integral_constant<int, 128>(), std::false_type());
 }
 
 }  // namespace tops
