@@ -481,3 +481,15 @@ def test_window_attention_strides(device, dtype, lay, which):
     ref.assert_within(out, *want["out"], "out")
     for name, got in zip(("dq", "dk", "dv"), window_attn.backward(d, q, k, v, out, lse, window=(40, 9), sinks=3)):
         ref.assert_within(got, *want[name], name)
+
+
+def test_flags_without_a_truth_value():
+    """An error of the argument's own, not of an interpreter that finds one left behind."""
+    both = torch.ones(2)
+    q, pos, f, a = torch.zeros(1, 4, 2, 32), torch.zeros(1, 1, 4, dtype=torch.int32), torch.ones(16), torch.zeros(16).int()
+    x, w = torch.zeros(4, 64), torch.zeros(4, 4)
+    for call in (lambda: rotary.forward(q, None, pos, inv_freq=f, axis=a, interleaved=both),
+                 lambda: gated_norm.forward(x, x, post_norm=both), lambda: gated_norm.forward(x, x, pre_norm=both),
+                 lambda: gated_norm.backward(x, x, x, x, None, w, post_norm=both)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            call()

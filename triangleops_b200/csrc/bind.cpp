@@ -48,6 +48,11 @@ int64_t whole(PyObject* o) {
   if (v == -1 && PyErr_Occurred()) throw Refused();
   return v;
 }
+int flag(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Refused();
+  return v;
+}
 double real(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw Refused();
@@ -354,7 +359,7 @@ struct Norm {
 PyObject* gated_norm_forward(PyObject* const* a) {
   const Tensor x = tensor(a[0]), y = tensor(a[1]), gate = maybe(a[2]);
   const Norm s(x, y, gate, a + 3, a[8]);
-  const int post = PyObject_IsTrue(a[9]), pre = PyObject_IsTrue(a[10]);
+  const int post = flag(a[9]), pre = flag(a[10]);
   require_cuda(x);
   const c10::cuda::CUDAGuard guard(x.device());
   const Tensor h = like(x), n = pre ? like(x) : Tensor();
@@ -377,7 +382,7 @@ PyObject* gated_norm_backward(PyObject* const* a) {
   const Tensor dh = maybe(a[0]), dn = maybe(a[1]), x = tensor(a[2]), y = tensor(a[3]), gate = maybe(a[4]),
                stats = tensor(a[5]);
   const Norm s(x, y, gate, a + 6, a[11]);
-  const int post = PyObject_IsTrue(a[12]), pre = PyObject_IsTrue(a[13]);
+  const int post = flag(a[12]), pre = flag(a[13]);
   for (const Tensor* d : {&dh, &dn})
     if (d->defined()) {
       must(d->sizes() == x.sizes() && d->device() == x.device(), "dh and dn must be like x");
@@ -419,7 +424,7 @@ PyObject* rotary(PyObject* const* a) {
   Tensor q = tensor(a[0]), k = maybe(a[1]);
   const Tensor pos = tensor(a[2]);
   Tensor freq = tensor(a[3]), axis = tensor(a[4]);
-  const int dt = dtype_code(q);
+  const int dt = dtype_code(q), interleaved = flag(a[5]), negate = flag(a[6]);
   must(q.dim() == 4, "q must be (B, N, H, D)");
   const int64_t B = q.size(0), N = q.size(1), Hq = q.size(2), D = q.size(3);
   must(freq.dim() == 1 && freq.size(0) > 0 && 2 * freq.size(0) <= D, "inv_freq must be (P,) with 0 < 2P <= D");
@@ -450,9 +455,9 @@ PyObject* rotary(PyObject* const* a) {
   if (k.defined())
     for (int i = 0; i < 3; ++i) st[3 + i] = k.stride(i);
   const int64_t ps[3] = {pos.stride(0), pos.stride(1), pos.stride(2)};
-  check(tops_rotary(dt, B, N, Hq, Hk, D, freq.size(0), pos.size(0), PyObject_IsTrue(a[5]), PyObject_IsTrue(a[6]), ptr(q),
-                    ptr(k), st, ptr(pos), wide, ps, static_cast<const float*>(ptr(freq)),
-                    static_cast<const int32_t*>(ptr(axis)), out_ptr(qo), out_ptr(ko), stream_of(q)),
+  check(tops_rotary(dt, B, N, Hq, Hk, D, freq.size(0), pos.size(0), interleaved, negate, ptr(q), ptr(k), st, ptr(pos),
+                    wide, ps, static_cast<const float*>(ptr(freq)), static_cast<const int32_t*>(ptr(axis)), out_ptr(qo),
+                    out_ptr(ko), stream_of(q)),
         "tops_rotary");
   return give_tuple(qo, ko);
 }
