@@ -18,6 +18,8 @@
 // S and dP are computed in both (7 products for the 5 of one that adds dQ up in memory by
 // atomics): nothing is added in an order that changes, and dS is not stored.
 //
+// delta comes from `out` as the forward stored it: O's rounding to the IO dtype enters dS, times P.
+//
 // KV walks the query heads of its key head one after the other, so the sum over a shared head's
 // queries stays in TMEM. The queries that see a tile's sinks only as sinks, all those past its window,
 // are the work of further, shorter blocks behind the tiles' own (a quarter of their length, so that
@@ -28,7 +30,8 @@
 // at a power of two of their size: P at 2^14 times, which its exponent takes along, and dS at 2^14 / 2^e
 // times with 2^e above the largest |dP - delta| that there can be, 2 max |dO_i| max |v_j| over the queries
 // that see a key and the keys that a query may see; the statistics' kernel finds both. The results'
-// factors take the powers out again. bf16 has the range of the sums.
+// factors take the powers out again (2 x 4096 queries as above: 214 us without, 221 so; 1024 queries of 4
+// heads 9.7 and 13.6, the clearing of the two maxima being one more node). bf16 has the range of the sums.
 //
 // Masked keys: P and dS are replaced by 0, and (Q) their rows of the k tile zeroed in shared memory
 // before dS k, so that what they hold reaches nothing. A query that sees nothing, and one past the

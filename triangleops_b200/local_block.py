@@ -11,7 +11,8 @@ Each block updates a residual stream s (B, N, C) twice:
 so a block is two fused norms, one rotary, one attention and four library products.
 :func:`forward` is differentiable in everything and takes whole sequences; :func:`step` takes
 one token for each sequence against the keys and values kept in :func:`caches`, and gives what
-:func:`forward` with the causal window gives at that token. No counterpart in the reference.
+:func:`forward` with the causal window gives at that token. :func:`forward` fills no caches: a
+sequence enters them token by token. No counterpart in the reference.
 """
 
 from __future__ import annotations

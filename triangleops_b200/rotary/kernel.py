@@ -6,7 +6,8 @@ Frequency f belongs to one axis of the positions; its pair of channels turns by
     (a, b) -> (a cos - b sin, a sin + b cos)
 
 Pairs are channels (f, D/2 + f), or (2f, 2f + 1) with ``interleaved``. There are
-P <= D/2 frequencies; channels of no pair are copied. Queries and keys go in one launch, an
+P <= D/2 frequencies; channels of no pair are copied. (A partial turn that pairs f with P + f within
+the first 2P channels is another form: turn ``q[..., :2 * P]``, a strided view, as heads of 2P.) Queries and keys go in one launch, an
 angle is formed in 64 bits. No counterpart in the reference.
 """
 

@@ -11,7 +11,14 @@ the keys) and sees key j where
 ``(W - 1, 0)``. The first ``sinks`` keys stay visible from any distance to their right.
 Several query heads may share a key head (Hq a multiple of Hkv). A query that sees no key
 gets zeros, log-sum-exp -inf, and passes no gradient; what masked keys hold (NaN and
-infinity too) reaches nothing.
+infinity too) reaches nothing, nor does what such a query and its gradient hold. A key that is
+not masked must be finite, seen or not: in :func:`forward` and :func:`backward` a tile's other
+queries multiply it by a probability of zero. (:func:`decode` reads only the keys that are
+seen.)
+
+In 16 bits P enters its products rounded once to the IO dtype and dS as two parts of it; in f16
+both are held at powers of two of their size there, so that small probabilities and gradients of any
+size keep their digits. Sums, maxima and statistics are fp32.
 
 No counterpart in the reference, whose attentions are dense.
 """
