@@ -493,3 +493,27 @@ def test_flags_without_a_truth_value():
                  lambda: gated_norm.backward(x, x, x, x, None, w, post_norm=both)):
         with pytest.raises(RuntimeError, match="ambiguous"):
             call()
+
+
+def test_builds_of_two_processes_do_not_share_a_file(monkeypatch, tmp_path):
+    """Ranks that start together may all compile: each writes a file of its own and moves it into place whole."""
+    import os
+    import types
+
+    written = []
+
+    def compiler(cmd, **_):
+        written.append(cmd[cmd.index("-o") + 1])
+        with open(written[-1], "w") as f:
+            f.write(cmd[0])
+        return types.SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    for name in ("LIB_PATH", "BIND_PATH", "BIND_STAMP"):
+        monkeypatch.setattr(_build, name, str(tmp_path / name))
+    monkeypatch.setattr(_build.subprocess, "run", compiler)
+    for pid in (11, 12):
+        monkeypatch.setattr(os, "getpid", lambda pid=pid: pid)
+        _build.build(force=True)
+        _build.build_bind(force=True)
+    assert len(set(written)) == 4
+    assert sorted(os.listdir(tmp_path)) == ["BIND_PATH", "BIND_STAMP", "LIB_PATH"]

@@ -99,7 +99,7 @@ def build_bind(verbose: bool = False, force: bool = False) -> str:
 
     root = os.path.dirname(torch.__file__)
     cuda = os.environ.get("CUDA_HOME") or os.path.dirname(os.path.dirname(_nvcc()))
-    tmp = BIND_PATH + ".tmp"
+    tmp = f"{BIND_PATH}.{os.getpid()}.tmp"
     inc = (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            os.path.join(cuda, "include"), sysconfig.get_paths()["include"])
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
@@ -107,8 +107,9 @@ def build_bind(verbose: bool = False, force: bool = False) -> str:
            tmp, f"-L{HERE}", f"-l:{LIB_NAME}", f"-L{os.path.join(root, 'lib')}", "-ltorch_python", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"]
     _run(cmd, tmp, BIND_PATH, verbose)
-    with open(BIND_STAMP, "w") as f:
+    with open(tmp, "w") as f:
         f.write(_bind_against())
+    os.replace(tmp, BIND_STAMP)
     return BIND_PATH
 
 
@@ -116,7 +117,7 @@ def build(verbose: bool = False, force: bool = False, extra_flags: list[str] | N
     """Compile ``csrc/tops_all.cu`` into ``libtriangleops_b200.so`` (sm_100a)."""
     if not force and not needs_build():
         return LIB_PATH
-    tmp = LIB_PATH + ".tmp"
+    tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
     cmd = [_nvcc(), *NVCC_FLAGS, *(extra_flags or []), os.path.join(CSRC, "tops_all.cu"), "-o", tmp]
     _run(cmd, tmp, LIB_PATH, verbose)
     return LIB_PATH
